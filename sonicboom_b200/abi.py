@@ -100,6 +100,11 @@ CORE = {
     "sb_moe_join": ("i", "ppppfipippipiiiipis"),
     "sb_gemm_tc5_takes_angles": ("i", "iiiiiiiii"),
     "sb_rotation_table": ("i", "piipps"),
+    "sb_rope_store_e4m3": ("i", "piiiiiiipppppippipis"),
+    "sb_attention_e4m3_plain": ("i", "ppiippppippiiiiifs"),
+    "sb_page_tables": ("i", "ppippiipipiiiiipppppppps"),
+    "sb_page_advance": ("i", "ppipipips"),
+    "sb_page_release": ("i", "pippiipipis"),
     "sb_sample_params_size": ("i", ""),
     "sb_sample": ("i", "piippipps"),
     "sb_add_i32": ("i", "piis"),

@@ -1,0 +1,218 @@
+// The paged key/value cache in 8 bits: the write that ends a q|k|v product's work, and attention that reads it in its plainest
+// form.  Layout [page][k|v][head][position in page][head size] of e4m3 numbers (e4m3.cuh), scales float32 [page][k|v][head].
+#include "common.cuh"
+#include "e4m3.cuh"
+
+int sb_check_attention_args(const char* who, int n_rows, int n_q_heads, int n_kv_heads, int hd, int window, int page_size);
+
+namespace {
+
+// The sequence's page i, or -1 where it has none: beyond its list, given back, or no page of this cache.
+__device__ __forceinline__ int own_page(const int32_t* page_off, const int32_t* page_ids, int seq, int i, int n_pages) {
+  const int first = page_off[seq];
+  if (i < 0 || i >= page_off[seq + 1] - first) return -1;
+  const int page = page_ids[first + i];
+  return page < n_pages ? page : -1;
+}
+
+// -------------------------------------------------------------------------------------- store
+// One block: the new rows of one sequence that lie in one page, of one head (query heads, then k, then v heads).  So the page's
+// scale is decided where all its new values are at hand, with no order between blocks.
+// Rotation of the pair (a, b): a c - b s, a s + b c, each product and sum rounded on its own, as everywhere in this library.
+constexpr int STORE_THREADS = 128;
+
+struct StoreArgs {
+  const float *qkv, *angles;                     // [rows][(q heads + 2 kv heads) hd]; [rows][rot]: cosines, then sines
+  const int32_t *seq_row0, *seq_pos0, *page_off, *page_ids;
+  uint8_t* cache;
+  float* scales;
+  void* q_out;
+  int n_q_heads, n_kv_heads, hd, rot, page_size, n_pages;
+};
+
+template <typename TQ>
+__global__ void __launch_bounds__(STORE_THREADS) store_kernel(const StoreArgs a) {
+  __shared__ float warp_most[STORE_THREADS / 32];
+  sb_pdl_launch();
+  sb_pdl_wait();
+  const int seq = blockIdx.z, head = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int row0 = a.seq_row0[seq], n_new = a.seq_row0[seq + 1] - row0, pos0 = a.seq_pos0[seq];
+  if (n_new <= 0 || pos0 < 0) return;
+  const int nth = pos0 / a.page_size + blockIdx.x, start = nth * a.page_size;
+  const int lo = max(pos0, start), hi = min(pos0 + n_new, start + a.page_size);       // positions
+  if (lo >= hi) return;
+  const int width = (a.n_q_heads + 2 * a.n_kv_heads) * a.hd, half = a.rot >> 1;
+  const bool is_v = head >= a.n_q_heads + a.n_kv_heads;
+  auto value = [&](int pos, int e) {
+    const int row = row0 + pos - pos0;
+    const float* x = a.qkv + (size_t)row * width + (size_t)head * a.hd;
+    if (is_v || e >= a.rot) return x[e];
+    const float* turn = a.angles + (size_t)row * a.rot;
+    return e < half ? sb_rot_lo(x[e], x[e + half], turn[e], turn[half + e]) : sb_rot_hi(x[e - half], x[e], turn[e - half], turn[e]);
+  };
+  if (head < a.n_q_heads) {
+    for (int pos = lo + warp; pos < hi; pos += STORE_THREADS / 32)
+      for (int e = lane; e < a.hd; e += 32)
+        ((TQ*)a.q_out)[((size_t)(row0 + pos - pos0) * a.n_q_heads + head) * a.hd + e] = sb_from_f32<TQ>(value(pos, e));
+    return;
+  }
+  const int page = own_page(a.page_off, a.page_ids, seq, nth, a.n_pages);
+  if (page < 0) return;                          // no page of its own there: nothing is written
+  float most = 0.0f;
+  for (int pos = lo + warp; pos < hi; pos += STORE_THREADS / 32)
+    for (int e = lane; e < a.hd; e += 32) most = fmaxf(most, e4m3_size(value(pos, e)));
+  most = sb_warp_max(most);
+  if (lane == 0) warp_most[warp] = most;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < STORE_THREADS / 32; ++w) most = fmaxf(most, warp_most[w]);
+  const size_t block = (size_t)page * 2 * a.n_kv_heads + (head - a.n_q_heads);
+  uint8_t* dst = a.cache + block * a.page_size * a.hd;
+  int e2 = e4m3_exponent(most);
+  if (lo > start) {                              // the page holds tokens of earlier steps
+    const int before = exponent_of(a.scales[block]);
+    if (e2 > before) {
+      const float shrink = exp2f((float)(before - e2));
+      for (int i = 2 * tid; i < (lo - start) * a.hd; i += 2 * STORE_THREADS) {
+        const float2 v = e4m3x2_to_float2(*reinterpret_cast<const uint16_t*>(dst + i));
+        *reinterpret_cast<uint16_t*>(dst + i) = (uint16_t)to_e4m3x2(v.x, v.y, shrink);
+      }
+    } else {
+      e2 = before;
+    }
+  }
+  __syncthreads();                               // everybody has read the scale
+  if (tid == 0) a.scales[block] = exp2_int(e2);
+  const float inverse = exp2_int(-e2);
+  for (int pos = lo + warp; pos < hi; pos += STORE_THREADS / 32)
+    for (int e = 2 * lane; e < a.hd; e += 64)
+      *reinterpret_cast<uint16_t*>(dst + (size_t)(pos - start) * a.hd + e) = (uint16_t)to_e4m3x2(value(pos, e), value(pos, e + 1), inverse);
+}
+
+// -------------------------------------------------------------------------------------- plain attention
+// One block per (row, query head), float32 arithmetic; chunks of 256 keys at absolute positions, merged in ascending order.
+constexpr int PLAIN_THREADS = 128, PLAIN_CHUNK = 256, PLAIN_MAX_HD = 1024;
+
+template <typename TQ>
+__global__ void __launch_bounds__(PLAIN_THREADS)
+attention_kernel(const TQ* q, TQ* out, const int32_t* row_seq, const int32_t* row_pos, const int32_t* page_off, const int32_t* page_ids,
+                 int page_size, const uint8_t* cache, const float* scales, int n_pages, int n_q_heads, int n_kv_heads, int hd, int window,
+                 float scale) {
+  __shared__ float qs[PLAIN_MAX_HD], scores[PLAIN_CHUNK], shared[4];
+  sb_pdl_launch();
+  sb_pdl_wait();
+  const int t = blockIdx.x, h = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int kvh = h / (n_q_heads / n_kv_heads), pos = row_pos[t], seq = row_seq[t];
+  TQ* dst = out + ((size_t)t * n_q_heads + h) * hd;
+  if (pos < 0) return;                           // a row behind the last sequence: left as it is
+  const int n_own = page_off[seq + 1] - page_off[seq];
+  if (pos / page_size >= n_own) {                // a position without a page: zeros, nothing is read
+    for (int d = tid; d < hd; d += PLAIN_THREADS) dst[d] = sb_from_f32<TQ>(0.0f);
+    return;
+  }
+  auto block_of = [&](int key, int v) -> size_t {
+    const int page = min(max(page_ids[page_off[seq] + key / page_size], 0), n_pages - 1);
+    return ((size_t)page * 2 + v) * n_kv_heads + kvh;
+  };
+  for (int d = tid; d < hd; d += PLAIN_THREADS) qs[d] = sb_to_f32<TQ>(q[((size_t)t * n_q_heads + h) * hd + d]);
+  __syncthreads();
+  const int lo = window > 0 ? max(0, pos - window + 1) : 0;
+  float m = -INFINITY, l = 0.0f, acc[PLAIN_MAX_HD / PLAIN_THREADS] = {};
+  for (int first = lo / PLAIN_CHUNK * PLAIN_CHUNK; first <= pos; first += PLAIN_CHUNK) {
+    for (int j = first + warp; j < first + PLAIN_CHUNK; j += PLAIN_THREADS / 32) {
+      float s = -INFINITY;
+      if (j >= lo && j <= pos) {
+        const size_t b = block_of(j, 0);
+        const uint8_t* k = cache + (b * page_size + j % page_size) * hd;
+        float dot = 0.0f;
+        for (int d = lane; d < hd; d += 32) dot = fmaf(qs[d], e4m3x2_to_float2(k[d]).x, dot);
+        s = sb_warp_sum(dot) * scales[b] * scale;
+      }
+      if (lane == 0) scores[j - first] = s;
+    }
+    __syncthreads();
+    if (warp == 0) {
+      float cm = -INFINITY;
+      for (int i = lane; i < PLAIN_CHUNK; i += 32) cm = fmaxf(cm, scores[i]);
+      const float m_new = fmaxf(m, sb_warp_max(cm)), base = m_new == -INFINITY ? 0.0f : m_new;
+      float sum = 0.0f;
+      for (int i = lane; i < PLAIN_CHUNK; i += 32) {
+        const float p = expf(scores[i] - base);
+        scores[i] = p;
+        sum += p;
+      }
+      sum = sb_warp_sum(sum);
+      if (lane == 0) {
+        shared[0] = expf(m - base);
+        shared[1] = sum;
+      }
+      m = m_new;
+    }
+    __syncthreads();
+    const float alpha = shared[0];
+    l = l * alpha + shared[1];
+#pragma unroll
+    for (int i = 0; i < PLAIN_MAX_HD / PLAIN_THREADS; ++i) acc[i] *= alpha;
+    for (int j = max(first, lo); j <= min(first + PLAIN_CHUNK - 1, pos); ++j) {
+      const size_t b = block_of(j, 1);
+      const uint8_t* v = cache + (b * page_size + j % page_size) * hd;
+      const float p = scores[j - first] * scales[b];
+#pragma unroll
+      for (int i = 0; i < PLAIN_MAX_HD / PLAIN_THREADS; ++i) {
+        const int d = tid + i * PLAIN_THREADS;
+        if (d < hd) acc[i] = fmaf(p, e4m3x2_to_float2(v[d]).x, acc[i]);
+      }
+    }
+    __syncthreads();
+  }
+#pragma unroll
+  for (int i = 0; i < PLAIN_MAX_HD / PLAIN_THREADS; ++i) {
+    const int d = tid + i * PLAIN_THREADS;
+    if (d < hd) dst[d] = sb_from_f32<TQ>(acc[i] / l);
+  }
+}
+
+}  // namespace
+
+extern "C" int sb_rope_store_e4m3(const float* qkv, int n_rows, int n_seqs, int max_new, int n_q_heads, int n_kv_heads, int hd, int rot,
+                                  const float* angles, const int32_t* seq_row0, const int32_t* seq_pos0, const int32_t* page_off,
+                                  const int32_t* page_ids, int page_size, void* cache, float* scales, int n_pages, void* q_out, int q_dtype,
+                                  cudaStream_t stream) {
+  const char* who = "sb_rope_store_e4m3";
+  if (!qkv || !seq_row0 || !seq_pos0 || !page_off || !page_ids || !cache || !scales || !q_out) SB_FAIL(SB_ERR_ARG, "%s: an array is missing", who);
+  if (n_rows <= 0 || n_seqs <= 0 || max_new <= 0 || n_q_heads <= 0 || n_kv_heads <= 0 || page_size <= 0 || n_pages <= 0)
+    SB_FAIL(SB_ERR_ARG, "%s: rows=%d seqs=%d max_new=%d heads=%d/%d page=%d pages=%d", who, n_rows, n_seqs, max_new, n_q_heads, n_kv_heads,
+            page_size, n_pages);
+  if (hd <= 0 || (hd & 1) || rot < 0 || rot > hd || (rot & 1))
+    SB_FAIL(SB_ERR_ARG, "%s: rotary dims %d of head dim %d (both even, rotary dims at most the head dim)", who, rot, hd);
+  if (rot > 0 && !angles) SB_FAIL(SB_ERR_ARG, "%s: %d rotary dims without angles", who, rot);
+  if (!sb_valid_dtype(q_dtype)) SB_FAIL(SB_ERR_ARG, "%s: dtype code %d", who, q_dtype);
+  if (n_seqs > 65535 || n_q_heads + 2 * n_kv_heads > 65535)
+    SB_FAIL(SB_ERR_UNSUPPORTED, "%s: %d sequences, %d/%d heads", who, n_seqs, n_q_heads, n_kv_heads);
+  const StoreArgs a = {qkv, angles, seq_row0, seq_pos0, page_off, page_ids, (uint8_t*)cache, scales, q_out,
+                       n_q_heads, n_kv_heads, hd, rot, page_size, n_pages};
+  const dim3 grid((unsigned)(((long)max_new + 2 * page_size - 2) / page_size), n_q_heads + 2 * n_kv_heads, n_seqs);
+  SB_DISPATCH_DTYPE(q_dtype, TQ, { sb_launch<SB_K_ELEMENTWISE>(store_kernel<TQ>, grid, dim3(STORE_THREADS), 0, stream, a); });
+  SB_CHECK_LAUNCH(who);
+  return SB_OK;
+}
+
+extern "C" int sb_attention_e4m3_plain(const void* q, void* out, int act_dtype, int n_rows, const int32_t* row_seq, const int32_t* row_pos,
+                                       const int32_t* page_off, const int32_t* page_ids, int page_size, const void* cache,
+                                       const float* scales, int n_pages, int n_q_heads, int n_kv_heads, int hd, int window, float scale,
+                                       cudaStream_t stream) {
+  const char* who = "sb_attention_e4m3_plain";
+  if (int rc = sb_check_attention_args(who, n_rows, n_q_heads, n_kv_heads, hd, window, page_size)) return rc;
+  if (!q || !out || !row_seq || !row_pos || !page_off || !page_ids || !cache || !scales || n_pages <= 0)
+    SB_FAIL(SB_ERR_ARG, "%s: %d pages, or an array is missing", who, n_pages);
+  if (hd > PLAIN_MAX_HD) SB_FAIL(SB_ERR_UNSUPPORTED, "%s: head dim %d is above %d", who, hd, PLAIN_MAX_HD);
+  if (!sb_valid_dtype(act_dtype)) SB_FAIL(SB_ERR_ARG, "%s: dtype code %d", who, act_dtype);
+  if (n_q_heads > 65535) SB_FAIL(SB_ERR_UNSUPPORTED, "%s: %d heads", who, n_q_heads);
+  SB_DISPATCH_DTYPE(act_dtype, TQ, {
+    sb_launch<SB_K_OTHER>(attention_kernel<TQ>, dim3(n_rows, n_q_heads), dim3(PLAIN_THREADS), 0, stream, (const TQ*)q, (TQ*)out, row_seq,
+                          row_pos, page_off, page_ids, page_size, (const uint8_t*)cache, scales, n_pages, n_q_heads, n_kv_heads, hd, window,
+                          scale);
+  });
+  SB_CHECK_LAUNCH(who);
+  return SB_OK;
+}

@@ -487,6 +487,47 @@ int sb_advance_rows(int32_t* x, const int32_t* last, int n, sb_stream_t stream);
 int sb_random_normal(void* out, int out_dtype, size_t n, uint32_t key0, uint32_t key1, float mean,
                      float std, sb_stream_t stream);
 
+/* ---- the paged cache in 8 bits (see e4m3.cuh, cache_e4m3.cu) ----
+ * cache [n_pages][k|v][kv head][position in page][hd] of e4m3 numbers, scales float32 [n_pages][k|v][kv head], each a power of
+ * two: the smallest that keeps the page's largest number within e4m3's 448.  Infinities and NaN are stored as NaN.
+ *
+ * Rotates q and k of the rows [q | k | v] by angles [rows][rot] (cosines, then sines: sb_rotation_table's), writes q to q_out
+ * and k, v into the pages; rot 0: no rotation, angles may be null.  A page that holds tokens of earlier steps keeps them: its
+ * numbers are brought to the new scale where that is larger.  A position without a page in its own sequence's list writes
+ * nothing but its q; rows behind the last sequence are left as they are.  hd even. */
+int sb_rope_store_e4m3(const float* qkv, int n_rows, int n_seqs, int max_new, int n_q_heads, int n_kv_heads, int hd, int rot,
+                       const float* angles, const int32_t* seq_row0, const int32_t* seq_pos0, const int32_t* page_off,
+                       const int32_t* page_ids, int page_size, void* cache, float* scales, int n_pages, void* q_out, int q_dtype,
+                       sb_stream_t stream);
+/* sb_attention_plain over that cache: float32 arithmetic, any head size up to 1024; a row with a negative position is left as it is. */
+int sb_attention_e4m3_plain(const void* q, void* out, int act_dtype, int n_rows, const int32_t* row_seq, const int32_t* row_pos,
+                            const int32_t* page_off, const int32_t* page_ids, int page_size, const void* cache, const float* scales,
+                            int n_pages, int n_q_heads, int n_kv_heads, int hd, int window, float scale, sb_stream_t stream);
+
+/* ---- a step's tables from request lengths (see page_tables.cu) ----
+ * State: lengths [n_slots], table [n_slots][width] of page ids, the stack of free pages free [n_pages] with n_free [1] of them.
+ * Request i brings fresh[i] >= 0 tokens of the sequence in slots[i].  Written: seq_row0 [n_seqs + 1], seq_pos0 [n_seqs],
+ * row_seq, row_pos, row_slot [max_rows] (page * page_size + place; 0, -1, -1 in rows behind the last sequence),
+ * page_off [n_seqs + 1], page_ids [max_pages] (as far as page_off says), status [1], and new pages into table.  lengths and n_free
+ * stay: sb_page_advance records the step.  status: 0, or SbTablesStatus bits; then the tables describe no rows. */
+enum SbTablesStatus {
+  SB_TABLES_BAD_REQUEST = 1,   /* a slot that does not exist or is named twice, a negative number of tokens */
+  SB_TABLES_TOO_LONG = 2,      /* more tokens than max_new, max_len or a slot's pages */
+  SB_TABLES_ROWS = 4,          /* more rows than max_rows */
+  SB_TABLES_PAGE_LIST = 8,     /* more pages than max_pages */
+  SB_TABLES_NO_PAGES = 16      /* more new pages than are free */
+};
+int sb_page_tables(const int32_t* slots, const int32_t* fresh, int n_seqs, const int32_t* lengths, int32_t* table, int n_slots, int width,
+                   const int32_t* free, int n_pages, const int32_t* n_free, int page_size, int max_rows, int max_pages, int max_new,
+                   int max_len, int32_t* seq_row0, int32_t* seq_pos0, int32_t* row_seq, int32_t* row_pos, int32_t* row_slot,
+                   int32_t* page_off, int32_t* page_ids, int32_t* status, sb_stream_t stream);
+/* The step that these tables described has run: lengths grow, n_free shrinks (neither where status is not 0). */
+int sb_page_advance(const int32_t* slots, const int32_t* fresh, int n_seqs, int32_t* lengths, int n_slots, int32_t* n_free, int page_size,
+                    const int32_t* status, sb_stream_t stream);
+/* Sequences end: their pages go back on the stack, their lengths to 0. */
+int sb_page_release(const int32_t* slots, int n_seqs, int32_t* lengths, int32_t* table, int n_slots, int width, int32_t* free, int n_pages,
+                    int32_t* n_free, int page_size, sb_stream_t stream);
+
 /* ------------------------------------------------------------------ attention library */
 int sb_attention_head_dim(void);
 void sb_attention_force_mma(int mode);    /* 0 by size; 1 the mma.sync kernels; 2 the TMA decode kernel always */

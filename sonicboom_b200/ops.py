@@ -669,6 +669,156 @@ def attention_status(head_dim: int) -> int:
     return int(al.sb_attention_status()) if al is not None else -1
 
 
+# ---------------------------------------------------------------- the paged cache in 8 bits
+E4M3 = torch.float8_e4m3fn
+
+
+def _on_current_device(t, what) -> None:
+    index = t.device.index
+    if t.is_cuda and index != (_raw_device() if _raw_device is not None else torch.cuda.current_device()):
+        raise KernelError(f"{what}: tensors are on {t.device}, the current device is another: launches go to the current device's stream")
+
+
+def _check_e4m3(what, plan, g, cache, scales, n_kv_heads, head_dim, n_rows) -> None:
+    """What every kernel over an 8-bit cache asks of the plan and the cache."""
+    _on_current_device(cache, what)
+    assert cache.dtype == E4M3 and cache.dim() == 5 and tuple(cache.shape[1:]) == (2, n_kv_heads, g.page_size, head_dim), \
+        f"{what}: cache is {cache.dtype} {tuple(cache.shape)}, want {E4M3} [pages, 2, {n_kv_heads}, {g.page_size}, {head_dim}]"
+    assert scales.dtype == torch.float32 and scales.shape == cache.shape[:3], \
+        f"{what}: scales are {scales.dtype} {tuple(scales.shape)}, want float32 {tuple(cache.shape[:3])}"
+    assert n_rows == plan.n_rows, f"{what}: {n_rows} rows, the plan has {plan.n_rows}"
+    assert plan.seq_row0.numel() == g.page_off.numel() == plan.n_seqs + 1 and plan.seq_pos0.numel() == plan.n_seqs
+
+
+def rope_store_e4m3(qkv: torch.Tensor, n_q_heads: int, n_kv_heads: int, head_dim: int, rotary_dim: int,
+                    angles: torch.Tensor | None, plan, group_index: int, cache: torch.Tensor, scales: torch.Tensor,
+                    q_out: torch.Tensor) -> torch.Tensor:
+    """`rope_store` into a cache held in 8 bits: rotates q and k of the float32 rows [q | k | v] by `angles` (the
+    `rotation_table` of the plan's rows; None when `rotary_dim` is 0), writes q to q_out [rows, heads, hd] and k, v into the
+    plan's pages.
+
+    `cache` [page, k|v, kv head, place, hd] holds e4m3 numbers, `scales` float32 [page, k|v, kv head] what they stand for: value =
+    number * scale.  A scale is the smallest power of two that leaves no number of the page above 448; infinities and NaN do not
+    count for it and are stored as NaN.  A page that holds tokens of earlier steps keeps them: where the new ones need a larger
+    scale its older numbers go over to it, which rounds only what falls below e4m3's normal numbers.  A page's first token starts
+    its scale anew.  Rows behind the plan's last sequence are left as they are."""
+    n, g = qkv.shape[0], plan.groups[group_index]
+    _check_e4m3("rope_store_e4m3", plan, g, cache, scales, n_kv_heads, head_dim, n)
+    assert qkv.dtype == torch.float32 and qkv.dim() == 2 and qkv.shape[1] == (n_q_heads + 2 * n_kv_heads) * head_dim
+    assert q_out.numel() == n * n_q_heads * head_dim
+    if angles is not None:
+        assert angles.dtype == torch.float32 and tuple(angles.shape) == (n, rotary_dim)
+    _check(lib().sb_rope_store_e4m3(
+        _ptr(qkv), n, plan.n_seqs, plan.max_new, n_q_heads, n_kv_heads, head_dim, rotary_dim, _ptr(angles),
+        _i32(plan.seq_row0, "seq_row0"), _i32(plan.seq_pos0, "seq_pos0"), _i32(g.page_off, "page_off"), _i32(g.page_ids, "page_ids"),
+        g.page_size, _ptr(cache), _ptr(scales), cache.shape[0], _ptr(q_out), _code(q_out.dtype), _stream()), "rope_store_e4m3")
+    return q_out
+
+
+def attention_e4m3(q: torch.Tensor, out: torch.Tensor, plan, group_index: int, cache: torch.Tensor, scales: torch.Tensor,
+                   n_q_heads: int, n_kv_heads: int, head_dim: int, window: int, scale: float) -> torch.Tensor:
+    """`attention` of the step's rows over a cache held in 8 bits (see `rope_store_e4m3`): causal, grouped queries, with `window`
+    n > 0 only the last n keys.  q and out bfloat16 or float32, of one dtype.  Rows behind the plan's last sequence are left as
+    they are; a sequence whose positions have no pages gets zeros."""
+    n, g = q.shape[0], plan.groups[group_index]
+    _check_e4m3("attention_e4m3", plan, g, cache, scales, n_kv_heads, head_dim, n)
+    assert q.dtype == out.dtype and q.numel() == out.numel() == n * n_q_heads * head_dim
+    _check(lib().sb_attention_e4m3_plain(
+        _ptr(q), _ptr(out), _code(q.dtype), n, _i32(plan.row_seq, "row_seq"), _i32(plan.row_pos, "row_pos"),
+        _i32(g.page_off, "page_off"), _i32(g.page_ids, "page_ids"), g.page_size, _ptr(cache), _ptr(scales), cache.shape[0], n_q_heads,
+        n_kv_heads, head_dim, window, ctypes.c_float(scale), _stream()), "attention_e4m3 (plain kernel)")
+    return out
+
+
+# ---------------------------------------------------------------- a step's tables from request lengths
+class TableGroup:
+    """What a plan says of one group of cache entries: `page_ids[page_off[i]: page_off[i + 1]]` are sequence i's pages."""
+
+    def __init__(self, page_off, page_ids, page_size):
+        self.page_off, self.page_ids, self.page_size = page_off, page_ids, page_size
+
+
+class PageTables:
+    """The arrays that `page_tables` writes, with room for `max_seqs` requests, `max_rows` rows and `max_pages` pages of all
+    requests together: a plan that the kernels take.  Its addresses stay, so a captured graph may write and read it."""
+
+    def __init__(self, max_seqs: int, max_rows: int, max_pages: int, device, page_size: int = 64):
+        assert min(max_seqs, max_rows, max_pages, page_size) > 0
+        sizes = [max_seqs + 1, max_seqs, max_rows, max_rows, max_rows, max_seqs + 1, max_pages, 1]
+        starts = [0]
+        for n in sizes:
+            starts.append(starts[-1] + (n + 3) // 4 * 4)         # every array starts on 16 bytes
+        flat = torch.full((starts[-1],), -1, dtype=torch.int32, device=device)
+        (self.seq_row0, self.seq_pos0, self.row_seq, self.row_pos, self.row_slot, self.page_off, self.page_ids,
+         self.status) = (flat[a:a + n] for a, n in zip(starts, sizes))
+        self._pointers = [t.data_ptr() for t in (self.seq_row0, self.seq_pos0, self.row_seq, self.row_pos, self.row_slot,
+                                                 self.page_off, self.page_ids, self.status)]
+        self.seq_row0.zero_(), self.page_off.zero_(), self.status.zero_()
+        self.n_seqs, self.n_rows, self.max_pages, self.page_size, self.device = max_seqs, max_rows, max_pages, page_size, flat.device
+        self.max_new = self.max_len = 0
+        self.groups = [TableGroup(self.page_off, self.page_ids, page_size)]
+        self._scratch = None
+
+    def scratch(self, nbytes: int, device):
+        """Scratch memory shared by the step's kernels (made on first use, grown on demand); None when nothing is asked for."""
+        if nbytes <= 0:
+            return None
+        if self._scratch is None or self._scratch.numel() < nbytes:
+            self._scratch = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        return self._scratch
+
+    def check(self) -> None:
+        """Raises KernelError where the last `page_tables` described no rows.  Waits for the device."""
+        status = int(self.status.item())
+        if status:
+            why = [text for bit, text in ((1, "a slot that does not exist or is named twice, or a negative number of tokens"),
+                                          (2, "a request beyond max_new, max_len or a slot's pages"), (4, "more rows than there is room for"),
+                                          (8, "more pages than there is room for"), (16, "not enough free pages")) if status & bit]
+            raise KernelError("page_tables: " + "; ".join(why))
+
+
+def page_tables(slots: torch.Tensor, new: torch.Tensor, lengths: torch.Tensor, table: torch.Tensor, free: torch.Tensor,
+                n_free: torch.Tensor, tables: PageTables, max_new: int, max_len: int) -> PageTables:
+    """A step's plan made on the device: request i brings `new[i]` >= 0 tokens of the sequence in slot `slots[i]`, which holds
+    `lengths[slot]` tokens in the pages `table[slot]` [slots, pages of a slot]; pages that it needs beyond them are the next ones
+    of the stack `free[:n_free]`, its top first, in the order of the requests, and are written into `table` too.
+
+    `tables` gets seq_row0, seq_pos0, page_off, page_ids and, for every row, row_seq, row_pos and row_slot (page * page size +
+    place); rows behind the last sequence get 0, -1 and -1.  `max_new` and `max_len` bound every request's new tokens and its
+    length after them.  All or nothing: where a request cannot be met `tables.status` says why and the tables describe no rows
+    (`tables.check()` raises it).  Nothing is taken until `page_advance` records the step; called again before that, it gives the
+    same pages.  All arrays int32."""
+    n = tables.n_seqs
+    _on_current_device(lengths, "page_tables")
+    assert slots.numel() == new.numel() == n, f"page_tables: {slots.numel()} slots, {new.numel()} counts, tables for {n} requests"
+    assert table.dim() == 2 and lengths.numel() == table.shape[0] and n_free.numel() == 1 and tables.device == lengths.device
+    _check(lib().sb_page_tables(
+        _i32(slots, "slots"), _i32(new, "new"), n, _i32(lengths, "lengths"), _i32(table, "table"), table.shape[0], table.shape[1],
+        _i32(free, "free"), free.numel(), _i32(n_free, "n_free"), tables.page_size, tables.n_rows, tables.max_pages, max_new, max_len,
+        *tables._pointers, _stream()), "page_tables")
+    tables.max_new, tables.max_len = max_new, max_len
+    return tables
+
+
+def page_advance(slots: torch.Tensor, new: torch.Tensor, lengths: torch.Tensor, n_free: torch.Tensor, tables: PageTables) -> None:
+    """The step that `page_tables` of the same slots and counts described has run: its sequences grow, its pages are taken.
+    Changes nothing where the tables have a status."""
+    assert slots.numel() == new.numel() == tables.n_seqs and n_free.numel() == 1
+    _on_current_device(lengths, "page_advance")
+    _check(lib().sb_page_advance(_i32(slots, "slots"), _i32(new, "new"), tables.n_seqs, _i32(lengths, "lengths"), lengths.numel(),
+                                 _i32(n_free, "n_free"), tables.page_size, _i32(tables.status, "status"), _stream()), "page_advance")
+
+
+def page_release(slots: torch.Tensor, lengths: torch.Tensor, table: torch.Tensor, free: torch.Tensor, n_free: torch.Tensor,
+                 page_size: int = 64) -> None:
+    """The sequences in `slots` end: their pages go back on the stack and their lengths to 0."""
+    assert table.dim() == 2 and lengths.numel() == table.shape[0] and n_free.numel() == 1
+    _on_current_device(lengths, "page_release")
+    _check(lib().sb_page_release(_i32(slots, "slots"), slots.numel(), _i32(lengths, "lengths"), _i32(table, "table"), table.shape[0],
+                                 table.shape[1], _i32(free, "free"), free.numel(), _i32(n_free, "n_free"), page_size, _stream()),
+           "page_release")
+
+
 def sample_params_size() -> int:
     return lib().sb_sample_params_size()
 
