@@ -33,7 +33,7 @@ class BuildError(RuntimeError):
 
 # Sources that are compiled once per parameter value into libraries of their own, not into the
 # core library: {source: macro}.  The attention kernels are specialised by head size.
-VARIANT_SOURCES = {"attn_mma.cu": "SB_HD"}
+VARIANT_SOURCES = {"attn_mma.cu": "SB_HD", "attn_e4m3.cu": "SB_HD"}
 SHARED_SOURCES = ["error.cu"]            # linked into every library
 HEAD_DIMS = tuple(range(16, 257, 16))    # head sizes the attention kernels are written for
 
@@ -127,7 +127,7 @@ def build_attention(head_dim: int, force: bool = False, verbose: bool = True) ->
     if head_dim not in HEAD_DIMS:
         raise BuildError(f"the tensor-core attention kernels take head sizes in steps of 16 up to "
                          f"{HEAD_DIMS[-1]}, not {head_dim}")
-    srcs = [SRC_DIR / "attn_mma.cu"] + [SRC_DIR / s for s in SHARED_SOURCES]
+    srcs = [SRC_DIR / s for s in (*VARIANT_SOURCES, *SHARED_SOURCES)]
     return _build_lib(f"libsonicboom_b200_attn_hd{head_dim}.so", srcs, (f"-DSB_HD={head_dim}",),
                       force, verbose)
 

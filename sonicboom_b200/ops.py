@@ -716,13 +716,32 @@ def rope_store_e4m3(qkv: torch.Tensor, n_q_heads: int, n_kv_heads: int, head_dim
 
 
 def attention_e4m3(q: torch.Tensor, out: torch.Tensor, plan, group_index: int, cache: torch.Tensor, scales: torch.Tensor,
-                   n_q_heads: int, n_kv_heads: int, head_dim: int, window: int, scale: float) -> torch.Tensor:
+                   n_q_heads: int, n_kv_heads: int, head_dim: int, window: int, scale: float, kernel: str = "auto") -> torch.Tensor:
     """`attention` of the step's rows over a cache held in 8 bits (see `rope_store_e4m3`): causal, grouped queries, with `window`
     n > 0 only the last n keys.  q and out bfloat16 or float32, of one dtype.  Rows behind the plan's last sequence are left as
-    they are; a sequence whose positions have no pages gets zeros."""
+    they are; a sequence whose positions have no pages gets zeros.
+
+    bfloat16 at head sizes in steps of 16 up to 256 and pages of 64 keys runs on tensor cores (built for the head size at first
+    use); anything else, or `kernel="plain"`, runs the plain kernel."""
+    global LAUNCHES
     n, g = q.shape[0], plan.groups[group_index]
     _check_e4m3("attention_e4m3", plan, g, cache, scales, n_kv_heads, head_dim, n)
     assert q.dtype == out.dtype and q.numel() == out.numel() == n * n_q_heads * head_dim
+    if kernel not in ("auto", "plain"):
+        raise KernelError(f"attention_e4m3: unknown kernel {kernel!r}")
+    al = attention_lib(head_dim) if q.dtype == torch.bfloat16 and kernel == "auto" and g.page_size == 64 \
+        and (q.data_ptr() | cache.data_ptr() | out.data_ptr()) % 16 == 0 else None
+    if al is not None:
+        scratch = plan.scratch(int(al.sb_attention_e4m3_scratch_bytes(n, n_q_heads, plan.max_len)), q.device)
+        rc = al.sb_attention_e4m3(
+            _ptr(q), _ptr(out), n, plan.n_seqs, plan.max_new, plan.max_len, _i32(plan.seq_row0, "seq_row0"),
+            _i32(plan.seq_pos0, "seq_pos0"), _i32(g.page_off, "page_off"), _i32(g.page_ids, "page_ids"), g.page_size, _ptr(cache),
+            _ptr(scales), cache.shape[0], n_q_heads, n_kv_heads, head_dim, window, ctypes.c_float(scale), _ptr(scratch),
+            scratch.numel() if scratch is not None else 0, _stream())
+        if rc != 0:
+            raise KernelError(f"attention_e4m3: {al.sb_last_error().decode()}")
+        LAUNCHES += 1 if scratch is None else 2
+        return out
     _check(lib().sb_attention_e4m3_plain(
         _ptr(q), _ptr(out), _code(q.dtype), n, _i32(plan.row_seq, "row_seq"), _i32(plan.row_pos, "row_pos"),
         _i32(g.page_off, "page_off"), _i32(g.page_ids, "page_ids"), g.page_size, _ptr(cache), _ptr(scales), cache.shape[0], n_q_heads,
