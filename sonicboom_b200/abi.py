@@ -101,6 +101,7 @@ CORE = {
     "sb_gemm_tc5_takes_angles": ("i", "iiiiiiiii"),
     "sb_rotation_table": ("i", "piipps"),
     "sb_rope_store_e4m3": ("i", "piiiiiiipppppippipis"),
+    "sb_cache_e4m3_values": ("i", "ppiippiippiiiiipipps"),
     "sb_attention_e4m3_plain": ("i", "ppiippppippiiiiifs"),
     "sb_page_tables": ("i", "ppippiipipiiiiipppppppps"),
     "sb_page_advance": ("i", "ppipipips"),

@@ -89,6 +89,54 @@ __global__ void __launch_bounds__(STORE_THREADS) store_kernel(const StoreArgs a)
       *reinterpret_cast<uint16_t*>(dst + (size_t)(pos - start) * a.hd + e) = (uint16_t)to_e4m3x2(value(pos, e), value(pos, e + 1), inverse);
 }
 
+// -------------------------------------------------------------------------------------- values
+// The pages of a step's sequences as values in bfloat16 or float32, one after another as the plan lists them: [place in
+// page_ids][k|v][head][position][hd], with `numbers` for the page list that says so.  Exact in either type (a number has four bits, the scale is a power of two).  What no row of
+// the step sees (positions behind a sequence's end, before its first row's window) becomes 0, whatever the page holds there; pages
+// that lie wholly before the window are left out.  A sequence whose positions have no pages gets rows of zeros in `out`, which
+// the attention behind this kernel leaves alone.  One block a page and head; bound by memory (1 byte in, 2 or 4 out a value).
+// It lets its successor start at its end only: that may read the plan ahead of its own wait.
+constexpr int VALUES_THREADS = 128;
+
+template <typename T>
+__global__ void __launch_bounds__(VALUES_THREADS)
+values_kernel(const int32_t* seq_row0, const int32_t* seq_pos0, const int32_t* page_off, const int32_t* page_ids, int n_list, int page_size,
+              const uint8_t* cache, const float* scales, int n_pages, int n_kv_heads, int hd, int window, T* values,
+              int32_t* numbers, T* out, int out_width) {
+  sb_pdl_wait();
+  const int i = blockIdx.x, head = blockIdx.y, seq = blockIdx.z, tid = threadIdx.x;
+  const int row0 = seq_row0[seq], n_new = seq_row0[seq + 1] - row0, pos0 = seq_pos0[seq];
+  const int first = page_off[seq], n_own = page_off[seq + 1] - first, len = pos0 + n_new;
+  if (n_new <= 0) return;
+  if (pos0 < 0 || (len - 1) / page_size >= n_own) {
+    for (size_t at = ((size_t)i * gridDim.y + head) * VALUES_THREADS + tid; at < (size_t)n_new * out_width;
+         at += (size_t)gridDim.x * gridDim.y * VALUES_THREADS)
+      out[(size_t)row0 * out_width + at] = sb_from_f32<T>(0.0f);
+    return;
+  }
+  const int start = i * page_size, low = window > 0 ? max(0, pos0 - window + 1) : 0;
+  if (start >= len || first + i >= n_list) return;
+  if (head == 0 && tid == 0) numbers[first + i] = first + i;
+  if (start + page_size <= low) return;
+  const int page = min(max(page_ids[first + i], 0), n_pages - 1);
+  const size_t block = (size_t)page * gridDim.y + head;
+  const uint32_t* src = reinterpret_cast<const uint32_t*>(cache + block * page_size * hd);
+  T* dst = values + ((size_t)(first + i) * gridDim.y + head) * page_size * hd;
+  const float scale = scales[block];
+#pragma unroll 4
+  for (int w = tid; w < page_size * hd / 4; w += VALUES_THREADS) {
+    const int pos = start + 4 * w / hd;
+    const uint32_t v = pos >= low && pos < len ? src[w] : 0;
+    const float2 a = e4m3x2_to_float2(v & 0xffffu), b = e4m3x2_to_float2(v >> 16);
+    if constexpr (sizeof(T) == 2) {
+      const __nv_bfloat162 x = __floats2bfloat162_rn(a.x * scale, a.y * scale), y = __floats2bfloat162_rn(b.x * scale, b.y * scale);
+      *reinterpret_cast<uint2*>(dst + 4 * (size_t)w) = make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
+    } else {
+      *reinterpret_cast<float4*>(dst + 4 * (size_t)w) = make_float4(a.x * scale, a.y * scale, b.x * scale, b.y * scale);
+    }
+  }
+}
+
 // -------------------------------------------------------------------------------------- plain attention
 // One block per (row, query head), float32 arithmetic; chunks of 256 keys at absolute positions, merged in ascending order.
 constexpr int PLAIN_THREADS = 128, PLAIN_CHUNK = 256, PLAIN_MAX_HD = 1024;
@@ -193,6 +241,30 @@ extern "C" int sb_rope_store_e4m3(const float* qkv, int n_rows, int n_seqs, int 
                        n_q_heads, n_kv_heads, hd, rot, page_size, n_pages};
   const dim3 grid((unsigned)(((long)max_new + 2 * page_size - 2) / page_size), n_q_heads + 2 * n_kv_heads, n_seqs);
   SB_DISPATCH_DTYPE(q_dtype, TQ, { sb_launch<SB_K_ELEMENTWISE>(store_kernel<TQ>, grid, dim3(STORE_THREADS), 0, stream, a); });
+  SB_CHECK_LAUNCH(who);
+  return SB_OK;
+}
+
+extern "C" int sb_cache_e4m3_values(const int32_t* seq_row0, const int32_t* seq_pos0, int n_seqs, int max_len, const int32_t* page_off,
+                                    const int32_t* page_ids, int n_list, int page_size, const void* cache, const float* scales, int n_pages,
+                                    int n_q_heads, int n_kv_heads, int hd, int window, void* values, int dtype,
+                                    int32_t* numbers, void* out, cudaStream_t stream) {
+  const char* who = "sb_cache_e4m3_values";
+  if (!seq_row0 || !seq_pos0 || !page_off || !page_ids || !cache || !scales || !values || !numbers || !out)
+    SB_FAIL(SB_ERR_ARG, "%s: an array is missing", who);
+  if (n_seqs <= 0 || max_len <= 0 || n_list <= 0 || page_size <= 0 || n_pages <= 0 || n_q_heads <= 0 || n_kv_heads <= 0 || window < 0)
+    SB_FAIL(SB_ERR_ARG, "%s: seqs=%d max_len=%d list=%d page=%d pages=%d heads=%d/%d window=%d", who, n_seqs, max_len, n_list, page_size,
+            n_pages, n_q_heads, n_kv_heads, window);
+  if (hd <= 0 || hd % 4 || (((uintptr_t)cache | (uintptr_t)values) & 15))
+    SB_FAIL(SB_ERR_UNSUPPORTED, "%s: head size %d (a multiple of 4), or unaligned pages", who, hd);
+  if (!sb_valid_dtype(dtype)) SB_FAIL(SB_ERR_ARG, "%s: dtype code %d", who, dtype);
+  if (n_seqs > 65535 || n_kv_heads > 32767) SB_FAIL(SB_ERR_UNSUPPORTED, "%s: %d sequences, %d key/value heads", who, n_seqs, n_kv_heads);
+  const dim3 grid((max_len + page_size - 1) / page_size, 2 * n_kv_heads, n_seqs);
+  SB_DISPATCH_DTYPE(dtype, T, {
+    sb_launch<SB_K_ELEMENTWISE>(values_kernel<T>, grid, dim3(VALUES_THREADS), 0, stream, seq_row0, seq_pos0, page_off, page_ids, n_list,
+                                page_size, (const uint8_t*)cache, scales, n_pages, n_kv_heads, hd, window, (T*)values, numbers, (T*)out,
+                                n_q_heads * hd);
+  });
   SB_CHECK_LAUNCH(who);
   return SB_OK;
 }

@@ -715,22 +715,63 @@ def rope_store_e4m3(qkv: torch.Tensor, n_q_heads: int, n_kv_heads: int, head_dim
     return q_out
 
 
+E4M3_FEW_ROWS = 16               # rows (new tokens x heads) of one key/value head up to which pages are read as they are
+
+
+class _ValuesPlan:
+    """A plan whose pages lie one after another in scratch memory, for `attention`."""
+
+    def __init__(self, plan, group):
+        self.n_rows, self.n_seqs, self.max_new, self.max_len = plan.n_rows, plan.n_seqs, plan.max_new, plan.max_len
+        self.seq_row0, self.seq_pos0, self.row_seq, self.row_pos = plan.seq_row0, plan.seq_pos0, plan.row_seq, plan.row_pos
+        self.groups = [group]
+
+    def scratch(self, nbytes, device):
+        return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes > 0 else None
+
+
+def _attention_of_values(q, out, plan, g, cache, scales, n_q_heads, n_kv_heads, head_dim, window, scale):
+    """`attention_e4m3` by way of the step's pages as values of q's type."""
+    n_list = g.page_ids.numel()
+    nbytes = (n_list * cache[0].numel() * q.element_size() + 15) // 16 * 16
+    scratch = plan.scratch(nbytes + 4 * n_list, q.device)
+    values, numbers = scratch[:nbytes].view(q.dtype).view(n_list, *cache.shape[1:]), scratch[nbytes:nbytes + 4 * n_list].view(torch.int32)
+    _check(lib().sb_cache_e4m3_values(
+        _i32(plan.seq_row0, "seq_row0"), _i32(plan.seq_pos0, "seq_pos0"), plan.n_seqs, plan.max_len, _i32(g.page_off, "page_off"),
+        _i32(g.page_ids, "page_ids"), n_list, g.page_size, _ptr(cache), _ptr(scales), cache.shape[0], n_q_heads, n_kv_heads, head_dim,
+        window, _ptr(values), _code(q.dtype), _ptr(numbers), _ptr(out), _stream()), "attention_e4m3 (values)")
+    return attention(q, out, _ValuesPlan(plan, TableGroup(g.page_off, numbers, g.page_size)), 0, values, n_q_heads, n_kv_heads,
+                     head_dim, window, scale)
+
+
 def attention_e4m3(q: torch.Tensor, out: torch.Tensor, plan, group_index: int, cache: torch.Tensor, scales: torch.Tensor,
                    n_q_heads: int, n_kv_heads: int, head_dim: int, window: int, scale: float, kernel: str = "auto") -> torch.Tensor:
     """`attention` of the step's rows over a cache held in 8 bits (see `rope_store_e4m3`): causal, grouped queries, with `window`
     n > 0 only the last n keys.  q and out bfloat16 or float32, of one dtype.  Rows behind the plan's last sequence are left as
     they are; a sequence whose positions have no pages gets zeros.
 
-    bfloat16 at head sizes in steps of 16 up to 256 and pages of 64 keys runs on tensor cores (built for the head size at first
-    use); anything else, or `kernel="plain"`, runs the plain kernel."""
+    bfloat16 at head sizes in steps of 16 up to 256 and pages of 64 keys with few rows a sequence (up to E4M3_FEW_ROWS of a
+    key/value head) reads the pages on tensor cores.  More rows, and float32 at head sizes that are multiples of 4 up to 256, have
+    the step's pages brought to values first (exact, in the plan's scratch memory) and run `attention`.  Anything else, or
+    `kernel="plain"`, runs the plain kernel; `"few"` and `"values"` choose one of the others."""
     global LAUNCHES
     n, g = q.shape[0], plan.groups[group_index]
     _check_e4m3("attention_e4m3", plan, g, cache, scales, n_kv_heads, head_dim, n)
     assert q.dtype == out.dtype and q.numel() == out.numel() == n * n_q_heads * head_dim
-    if kernel not in ("auto", "plain"):
+    if kernel not in ("auto", "plain", "few", "values"):
         raise KernelError(f"attention_e4m3: unknown kernel {kernel!r}")
-    al = attention_lib(head_dim) if q.dtype == torch.bfloat16 and kernel == "auto" and g.page_size == 64 \
-        and (q.data_ptr() | cache.data_ptr() | out.data_ptr()) % 16 == 0 else None
+    aligned = (q.data_ptr() | cache.data_ptr() | out.data_ptr()) % 16 == 0
+    few = values = False
+    if kernel != "plain" and aligned:
+        few = q.dtype == torch.bfloat16 and head_dim in _build.HEAD_DIMS and g.page_size == 64
+        values = head_dim <= 256 and (few or (q.dtype == torch.float32 and head_dim % 4 == 0))
+        many = plan.max_new * (n_q_heads // n_kv_heads) > E4M3_FEW_ROWS
+        few = few and kernel != "values" and (kernel == "few" or not many)
+    if kernel in ("few", "values") and not (few or values):
+        raise KernelError(f"attention_e4m3: the kernel {kernel!r} does not take {q.dtype} at head size {head_dim}, pages of {g.page_size}")
+    if values and not few:
+        return _attention_of_values(q, out, plan, g, cache, scales, n_q_heads, n_kv_heads, head_dim, window, scale)
+    al = attention_lib(head_dim) if few else None
     if al is not None:
         scratch = plan.scratch(int(al.sb_attention_e4m3_scratch_bytes(n, n_q_heads, plan.max_len)), q.device)
         rc = al.sb_attention_e4m3(

@@ -68,6 +68,21 @@ def test_plain_attention_refusals(kw, code):
     assert attend(l, **kw) == code and b"sb_attention_e4m3_plain" in l.sb_last_error()
 
 
+def values(l, row0=P, pos0=P, seqs=2, max_len=100, off=P, ids=P, n_list=4, page=64, cache=P, scales=P, pages=8, hq=4, hkv=2, hd=64, window=0,
+           out=P, dtype=1, numbers=P, rows=P):
+    return l.sb_cache_e4m3_values(row0, pos0, seqs, max_len, off, ids, n_list, page, cache, scales, pages, hq, hkv, hd, window, out, dtype,
+                                  numbers, rows, None)
+
+
+@pytest.mark.parametrize("kw,code", [
+    (dict(row0=None), ARG), (dict(cache=None), ARG), (dict(out=None), ARG), (dict(numbers=None), ARG), (dict(rows=None), ARG),
+    (dict(seqs=0), ARG), (dict(max_len=0), ARG), (dict(n_list=0), ARG), (dict(page=0), ARG), (dict(pages=0), ARG), (dict(window=-1), ARG),
+    (dict(hd=66), UNSUPPORTED), (dict(out=P + 8), UNSUPPORTED), (dict(dtype=3), ARG), (dict(seqs=65536), UNSUPPORTED)])
+def test_values_refusals(kw, code):
+    l = ops.lib()
+    assert values(l, **kw) == code and b"sb_cache_e4m3_values" in l.sb_last_error()
+
+
 def tables(l, slots=P, new=P, n=4, lengths=P, table=P, n_slots=8, width=4, free=P, pages=32, n_free=P, page=64, max_rows=16, max_pages=16,
            max_new=4, max_len=256, outs=(P,) * 8):
     return l.sb_page_tables(slots, new, n, lengths, table, n_slots, width, free, pages, n_free, page, max_rows, max_pages, max_new, max_len,

@@ -164,7 +164,7 @@ def test_store_without_a_page_writes_nothing_but_q():
 
 
 # ------------------------------------------------------------------------------------------------ attention
-def attention_case(new, pos0, hq, hkv, hd, dtype, window=0, seed=0, spread=0.0, scale=None):
+def attention_case(new, pos0, hq, hkv, hd, dtype, window=0, seed=0, spread=0.0, scale=None, kernel="auto"):
     """Runs the operator on a cache that the plain form filled; compares every row."""
     g, rng = torch.Generator().manual_seed(seed + hd), random.Random(seed)
     lengths = [p + n for p, n in zip(pos0, new)]
@@ -189,7 +189,7 @@ def attention_case(new, pos0, hq, hkv, hd, dtype, window=0, seed=0, spread=0.0, 
     q = torch.randn(plan.n_rows, hq, hd, generator=g).to(dtype)
     out = torch.full((plan.n_rows, hq * hd), 5.0, dtype=dtype, device=DEV)
     scale = hd ** -0.5 if scale is None else scale
-    ops.attention_e4m3(q.to(DEV), out, plan, 0, cache, scales, hq, hkv, hd, window, scale)
+    ops.attention_e4m3(q.to(DEV), out, plan, 0, cache, scales, hq, hkv, hd, window, scale, kernel)
     got = out.cpu().double().view(plan.n_rows, hq, hd)
     at = 0
     for pages, p, n in zip(lists, pos0, new):
@@ -215,6 +215,16 @@ def test_attention_of_single_tokens(hq, hkv, hd, dtype):
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_attention_of_prompts(hq, hkv, hd, dtype):
     attention_case([70, 1, 0, 33, 2], [0, 130, 7, 100, 63], hq, hkv, hd, dtype)
+
+
+@pytest.mark.parametrize("hd", [16, 64, 128, 192, 256])
+@pytest.mark.parametrize("kernel", ["plain", "few", "values"])
+def test_attention_kernels_by_name(hd, kernel):
+    """The same calls through every kernel, those "auto" would not choose among them."""
+    attention_case([1, 3, 50], [70, 200, 20], 6, 2, hd, torch.bfloat16, kernel=kernel)
+    attention_case([1, 3, 50], [70, 200, 20], 6, 2, hd, torch.bfloat16, kernel=kernel, window=33)
+    if kernel != "few":
+        attention_case([1, 3, 50], [70, 200, 20], 6, 2, hd, torch.float32, kernel=kernel)
 
 
 @pytest.mark.parametrize("new,pos0", [([1, 1, 1], [500, 39, 40]), ([2, 2], [300, 63]), ([90, 1, 64], [0, 200, 129])])
