@@ -100,7 +100,7 @@ CORE = {
     "sb_moe_join": ("i", "ppppfipippipiiiipis"),
     "sb_gemm_tc5_takes_angles": ("i", "iiiiiiiii"),
     "sb_rotation_table": ("i", "piipps"),
-    "sb_rope_store_e4m3": ("i", "piiiiiiipppppippipis"),
+    "sb_rope_store_e4m3": ("i", "piiiiiiipppppippipiis"),
     "sb_cache_e4m3_values": ("i", "ppiippiippiiiiipipps"),
     "sb_attention_e4m3_plain": ("i", "ppiippppippiiiiifs"),
     "sb_page_tables": ("i", "ppippiipipiiiiipppppppps"),
@@ -120,7 +120,7 @@ ATTENTION = {
     "sb_attention_scratch_bytes": ("z", "iiiii"),
     "sb_attention": ("i", "ppiiippppipiiiifpzpiiiipzpfipis"),
     "sb_attention_e4m3_scratch_bytes": ("z", "iii"),
-    "sb_attention_e4m3": ("i", "ppiiiippppippiiiiifpzs"),
+    "sb_attention_e4m3": ("i", "ppiiiiippppippiiiiifpzs"),
     "sb_attention_decode_static": ("i", "ppiiippppipiiiifis"),
     "sb_attention_static_scratch_bytes": ("z", ""),
 }

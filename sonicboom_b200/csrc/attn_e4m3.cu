@@ -9,7 +9,9 @@
 // A tile's k index is a sum's order and nothing more, so a thread takes what lies together: 16 bytes of a key's row for four
 // k-steps of S, 16 bytes of each of four values' rows for eight tiles of O.  No shared memory, no barrier: a warp walks its
 // pages alone, with RING steps of 16 keys in flight.  e4m3 to half is exact.  q is brought to halves with a power of two for each
-// row, so its 8 bits stay; weights are rounded to halves (2^-11) after they were summed in float32.
+// row: a bfloat16's 8 bits stay.  Weights are rounded to halves (2^-11) after they were summed in float32, times 2^15 so that
+// small ones stay normal numbers.  For float32 rows q and the weights are two halves each, the second what the first left over
+// (together within 2^-24 of a row's largest value, 2^-22 of a weight), and every product two.
 //
 // Scales.  A page's key scale joins the score.  Its value scale 2^e joins the weight: with m the largest score so far and n the
 // largest of score + e, weights are exp2(s - m) in the sum and exp2(s + e - n) in the product with V, each at most 1, and
@@ -43,8 +45,8 @@ constexpr int STEP_WORDS = 2 * K_WORDS > 4 * V_WORDS ? 2 * K_WORDS : 4 * V_WORDS
 static_assert(HD % 16 == 0 && HD >= 16 && HD <= 256, "head size in steps of 16, at most 256");
 
 struct Args {
-  const bf16* q;                                 // [rows, n_q_heads, HD]
-  bf16* out;
+  const void* q;                                 // [rows, n_q_heads, HD]
+  void* out;
   const int32_t *seq_row0, *seq_pos0, *page_off, *page_ids;
   const uint8_t* cache;                          // [page][k|v][kv head][PAGE][HD]
   const float* scales;                           // [page][k|v][kv head]
@@ -159,8 +161,19 @@ __device__ __forceinline__ int dim_of(int d, int h, int g) {
   return base + 2 * g + h;
 }
 
+// A value as PARTS halves: itself rounded, then what that left over.
+template <int PARTS>
+__device__ __forceinline__ void to_halves(uint32_t (&f)[PARTS], float lo, float hi) {
+  f[0] = pack_half(lo, hi);
+  if constexpr (PARTS == 2) {
+    const float2 first = __half22float2(*reinterpret_cast<const __half2*>(&f[0]));
+    f[1] = pack_half(lo - first.x, hi - first.y);
+  }
+}
+
 // A row of q as the B operand of S^T, in the keys' order of k, over 2^x; returns 2^x, the row's largest exponent.
-__device__ __forceinline__ float load_query(uint32_t (&f)[HD / 16][2], const bf16* row, bool valid, int t) {
+template <typename T, int PARTS>
+__device__ __forceinline__ float load_query(uint32_t (&f)[HD / 16][2][PARTS], const T* row, bool valid, int t) {
   float v[HD / 4];
   float most = 0.0f;
 #pragma unroll
@@ -168,12 +181,18 @@ __device__ __forceinline__ float load_query(uint32_t (&f)[HD / 16][2], const bf1
     const int c = i / 4, rest = HD / 64 * 4;
     const int dim = i < rest ? 64 * c + 16 * t + 4 * (i % 4)
                     : N32 && i < rest + 2 ? HD / 64 * 64 + 8 * t + 4 * (i - rest) : HD - 16 + 4 * t;
-    uint2 raw = make_uint2(0u, 0u);
-    if (valid) raw = *reinterpret_cast<const uint2*>(row + dim);
-    v[4 * i] = __uint_as_float(raw.x << 16);
-    v[4 * i + 1] = __uint_as_float(raw.x & 0xffff0000u);
-    v[4 * i + 2] = __uint_as_float(raw.y << 16);
-    v[4 * i + 3] = __uint_as_float(raw.y & 0xffff0000u);
+    if constexpr (sizeof(T) == 2) {
+      uint2 raw = make_uint2(0u, 0u);
+      if (valid) raw = *reinterpret_cast<const uint2*>(row + dim);
+      v[4 * i] = __uint_as_float(raw.x << 16);
+      v[4 * i + 1] = __uint_as_float(raw.x & 0xffff0000u);
+      v[4 * i + 2] = __uint_as_float(raw.y << 16);
+      v[4 * i + 3] = __uint_as_float(raw.y & 0xffff0000u);
+    } else {
+      float4 raw = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      if (valid) raw = *reinterpret_cast<const float4*>(row + dim);
+      v[4 * i] = raw.x; v[4 * i + 1] = raw.y; v[4 * i + 2] = raw.z; v[4 * i + 3] = raw.w;
+    }
 #pragma unroll
     for (int j = 0; j < 4; ++j) most = fmaxf(most, fabsf(v[4 * i + j]));
   }
@@ -183,8 +202,8 @@ __device__ __forceinline__ float load_query(uint32_t (&f)[HD / 16][2], const bf1
   const float inverse = exp2_int(-x);
 #pragma unroll
   for (int i = 0; i < HD / 16; ++i) {
-    f[i][0] = pack_half(v[4 * i] * inverse, v[4 * i + 1] * inverse);
-    f[i][1] = pack_half(v[4 * i + 2] * inverse, v[4 * i + 3] * inverse);
+    to_halves<PARTS>(f[i][0], v[4 * i] * inverse, v[4 * i + 1] * inverse);
+    to_halves<PARTS>(f[i][1], v[4 * i + 2] * inverse, v[4 * i + 3] * inverse);
   }
   return exp2_int(x);
 }
@@ -193,13 +212,15 @@ __device__ __forceinline__ float load_query(uint32_t (&f)[HD / 16][2], const bf1
 __device__ __forceinline__ uint32_t nan_bytes(uint32_t v) { return __vcmpeq4(v & 0x7f7f7f7fu, 0x7f7f7f7fu); }
 
 // O^T += V^T P^T of 16 keys.
-template <int NT>
-__device__ __forceinline__ void values_step(float (&o)[NT][HD / 16][4], const uint32_t (&w)[STEP_WORDS], const uint32_t (&p)[NT][2]) {
+template <int NT, int PARTS>
+__device__ __forceinline__ void values_step(float (&o)[NT][HD / 16][4], const uint32_t (&w)[STEP_WORDS], const uint32_t (&p)[NT][2][PARTS]) {
   auto tile = [&](int d, uint32_t a01, uint32_t a23) {       // keys 2t, 2t+1 and 2t+8, 2t+9 of two dims, bytes in pairs
     const uint32_t a0 = e4m3x2_to_half2(a01 & 0xffffu), a1 = e4m3x2_to_half2(a01 >> 16);
     const uint32_t a2 = e4m3x2_to_half2(a23 & 0xffffu), a3 = e4m3x2_to_half2(a23 >> 16);
 #pragma unroll
-    for (int n = 0; n < NT; ++n) mma_f16(o[n][d], a0, a1, a2, a3, p[n][0], p[n][1]);
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int j = 0; j < PARTS; ++j) mma_f16(o[n][d], a0, a1, a2, a3, p[n][0][j], p[n][1][j]);
   };
 #pragma unroll
   for (int i = 0; i < V_WORDS; ++i) {
@@ -209,9 +230,19 @@ __device__ __forceinline__ void values_step(float (&o)[NT][HD / 16][4], const ui
   }
 }
 
-template <int NT>
-__global__ void __launch_bounds__(WARPS * 32, HD <= 128 && NT == 1 ? 3 : 2) attn_e4m3_kernel(const Args a) {
-  constexpr int ROWS = 8 * NT;
+__device__ __forceinline__ void store_row(bf16* dst, float4 v) {
+  const __nv_bfloat162 lo = __floats2bfloat162_rn(v.x, v.y), hi = __floats2bfloat162_rn(v.z, v.w);
+  *reinterpret_cast<uint2*>(dst) = make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+}
+__device__ __forceinline__ void store_row(float* dst, float4 v) { *reinterpret_cast<float4*>(dst) = v; }
+
+constexpr float WEIGHT_BITS = 15.0f;             // weights as halves are at most 2^15
+
+template <int NT, typename T>
+__global__ void __launch_bounds__(WARPS * 32, HD <= 128 && NT == 1 && sizeof(T) == 2 ? 3 : 2) attn_e4m3_kernel(const Args a) {
+  constexpr int ROWS = 8 * NT, PARTS = sizeof(T) / 2;
+  const T* const q = (const T*)a.q;
+  T* const out = (T*)a.out;
   __shared__ __align__(16) float part[WARPS][ROWS][PART];
   __shared__ float stat_m[WARPS][ROWS], stat_l[WARPS][ROWS], stat_n[WARPS][ROWS];
   sb_pdl_wait();
@@ -226,7 +257,7 @@ __global__ void __launch_bounds__(WARPS * 32, HD <= 128 && NT == 1 ? 3 : 2) attn
   if (!sq.reads) {                               // zeros; no page is read
     if (split == 0)
       for (int i = tid; i < min(ROWS, R - row_base) * (HD / 4); i += WARPS * 32)
-        *reinterpret_cast<uint2*>(a.out + row_at(row_base + i / (HD / 4)) * HD + 4 * (i % (HD / 4))) = make_uint2(0u, 0u);
+        store_row(out + row_at(row_base + i / (HD / 4)) * HD + 4 * (i % (HD / 4)), make_float4(0.0f, 0.0f, 0.0f, 0.0f));
     return;
   }
   if (split < sq.split_lo || split > sq.split_hi) return;
@@ -238,12 +269,12 @@ __global__ void __launch_bounds__(WARPS * 32, HD <= 128 && NT == 1 ? 3 : 2) attn
   const int tile_lo = max(split * sq.sp, low / PAGE), tile_hi = min(split * sq.sp + sq.sp - 1, last_pos / PAGE);
   const int32_t* pages = a.page_ids + a.page_off[b];
 
-  uint32_t qf[NT][HD / 16][2];
+  uint32_t qf[NT][HD / 16][2][PARTS];
   float fac[NT][2];                              // of rows 2t, 2t + 1: 2^x scale log2(e)
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
     const int r = row_base + 8 * n + g;
-    const float f = load_query(qf[n], a.q + row_at(min(r, R - 1)) * HD, r < R, t) * a.scale_log2;
+    const float f = load_query<T, PARTS>(qf[n], q + row_at(min(r, R - 1)) * HD, r < R, t) * a.scale_log2;
     fac[n][0] = __shfl_sync(0xffffffffu, f, 8 * t);
     fac[n][1] = __shfl_sync(0xffffffffu, f, 8 * t + 4);
   }
@@ -293,14 +324,16 @@ __global__ void __launch_bounds__(WARPS * 32, HD <= 128 && NT == 1 ? 3 : 2) attn
           const uint32_t a0 = e4m3x2_to_half2(x & 0xffffu), a1 = e4m3x2_to_half2(y & 0xffffu);
           const uint32_t a2 = e4m3x2_to_half2(x >> 16), a3 = e4m3x2_to_half2(y >> 16);
 #pragma unroll
-          for (int n = 0; n < NT; ++n) mma_f16(s[n][sub], a0, a1, a2, a3, qf[n][i][0], qf[n][i][1]);
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int j = 0; j < PARTS; ++j) mma_f16(s[n][sub], a0, a1, a2, a3, qf[n][i][0][j], qf[n][i][1][j]);
         }
         if (sub + RING < 8) issue(ring[sub % RING], bytes, sub + RING);
         else if (more) issue(ring[sub % RING], next_bytes, sub + RING - 8);
       }
       const int key0 = tile * PAGE;
       const bool whole = key0 + PAGE - 1 <= first_pos && key0 >= high_low;      // every row sees every key
-      uint32_t p[NT][4][2];
+      uint32_t p[4][NT][2][PARTS];
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         float most[2] = {-INFINITY, -INFINITY};
@@ -325,7 +358,7 @@ __global__ void __launch_bounds__(WARPS * 32, HD <= 128 && NT == 1 ? 3 : 2) attn
           const float m_at = m_new == -INFINITY ? 0.0f : m_new, ref_at = ref_new == -INFINITY ? 0.0f : ref_new;   // nothing seen: weights 0
           l[n][r] *= exp2f(m[n][r] - m_at);
           shrink[r] = exp2f(ref[n][r] - ref_at);
-          const float shift = (float)e - ref_at;
+          const float shift = (float)e - ref_at + WEIGHT_BITS;
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             float& v = s[n][i >> 1][2 * (i & 1) + r];
@@ -344,8 +377,13 @@ __global__ void __launch_bounds__(WARPS * 32, HD <= 128 && NT == 1 ? 3 : 2) attn
         }
 #pragma unroll
         for (int sub = 0; sub < 4; ++sub) {
-          p[n][sub][0] = transpose8x8(pack_half(s[n][sub][0], s[n][sub][1]));
-          p[n][sub][1] = transpose8x8(pack_half(s[n][sub][2], s[n][sub][3]));
+          to_halves<PARTS>(p[sub][n][0], s[n][sub][0], s[n][sub][1]);
+          to_halves<PARTS>(p[sub][n][1], s[n][sub][2], s[n][sub][3]);
+#pragma unroll
+          for (int j = 0; j < PARTS; ++j) {
+            p[sub][n][0][j] = transpose8x8(p[sub][n][0][j]);
+            p[sub][n][1][j] = transpose8x8(p[sub][n][1][j]);
+          }
         }
       }
 #pragma unroll
@@ -367,7 +405,7 @@ __global__ void __launch_bounds__(WARPS * 32, HD <= 128 && NT == 1 ? 3 : 2) attn
             }
           }
           if (__any_sync(0xffffffffu, nans)) {
-            uint32_t is_nan[STEP_WORDS], sees[NT][2];
+            uint32_t is_nan[STEP_WORDS], sees[NT][2][1];
 #pragma unroll
             for (int i = 0; i < 4 * V_WORDS; ++i) {
               const uint32_t f = nan_bytes(w[i]);
@@ -381,10 +419,10 @@ __global__ void __launch_bounds__(WARPS * 32, HD <= 128 && NT == 1 ? 3 : 2) attn
 #pragma unroll
               for (int h = 0; h < 2; ++h) {
                 const int key = key0 + 16 * sub + 2 * t + 8 * h;
-                sees[n][h] = (key <= pos && key >= lo ? 0x3c00u : 0u) | (key + 1 <= pos && key + 1 >= lo ? 0x3c000000u : 0u);
+                sees[n][h][0] = (key <= pos && key >= lo ? 0x3c00u : 0u) | (key + 1 <= pos && key + 1 >= lo ? 0x3c000000u : 0u);
               }
             }
-            values_step<NT>(count, is_nan, sees);
+            values_step<NT, 1>(count, is_nan, sees);
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -394,10 +432,7 @@ __global__ void __launch_bounds__(WARPS * 32, HD <= 128 && NT == 1 ? 3 : 2) attn
                   if (count[n][d][i] > 0.0f) o[n][d][i] = NAN;
           }
         }
-        uint32_t pn[NT][2];
-#pragma unroll
-        for (int n = 0; n < NT; ++n) pn[n][0] = p[n][sub][0], pn[n][1] = p[n][sub][1];
-        values_step<NT>(o, w, pn);
+        values_step<NT, PARTS>(o, w, p[sub]);
         if (sub + 4 + RING < 8) issue(w, bytes, sub + 4 + RING);
         else if (more) issue(w, next_bytes, sub + 4 + RING - 8);
       }
@@ -422,7 +457,7 @@ __global__ void __launch_bounds__(WARPS * 32, HD <= 128 && NT == 1 ? 3 : 2) attn
       if (g == 0) {
         stat_m[warp][row] = m[n][r];
         stat_l[warp][row] = l[n][r];
-        stat_n[warp][row] = ref[n][r];
+        stat_n[warp][row] = ref[n][r] - WEIGHT_BITS;
       }
     }
   }
@@ -446,9 +481,7 @@ __global__ void __launch_bounds__(WARPS * 32, HD <= 128 && NT == 1 ? 3 : 2) attn
     const size_t at_row = row_at(row_base + row);
     if (single) {
       const float inv = 1.0f / sum;
-      const __nv_bfloat162 lo = __floats2bfloat162_rn(acc.x * inv, acc.y * inv), hi = __floats2bfloat162_rn(acc.z * inv, acc.w * inv);
-      *reinterpret_cast<uint2*>(a.out + at_row * HD + c) =
-          make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+      store_row(out + at_row * HD + c, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
     } else {
       float* dst = a.scratch + (at_row * a.n_splits + split) * PART;
       *reinterpret_cast<float4*>(dst + c) = acc;
@@ -462,6 +495,7 @@ __global__ void __launch_bounds__(WARPS * 32, HD <= 128 && NT == 1 ? 3 : 2) attn
 // on their number alone.
 constexpr int GROUPS = 4;
 constexpr int MERGE_THREADS = (HD / 4) * GROUPS;
+template <typename T>
 __global__ void __launch_bounds__(MERGE_THREADS) attn_e4m3_merge_kernel(const Args a) {
   extern __shared__ __align__(16) float weights[];                  // [n_splits]
   __shared__ __align__(16) float sums[GROUPS][HD];
@@ -506,9 +540,7 @@ __global__ void __launch_bounds__(MERGE_THREADS) attn_e4m3_merge_kernel(const Ar
     acc.x += v.x; acc.y += v.y; acc.z += v.z; acc.w += v.w;
   }
   const float inv = 1.0f / (((den[0] + den[1]) + den[2]) + den[3]);
-  const __nv_bfloat162 lo = __floats2bfloat162_rn(acc.x * inv, acc.y * inv), hi = __floats2bfloat162_rn(acc.z * inv, acc.w * inv);
-  *reinterpret_cast<uint2*>(a.out + at_row * HD + c) =
-      make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+  store_row((T*)a.out + at_row * HD + c, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
 }
 
 }  // namespace
@@ -518,7 +550,7 @@ extern "C" size_t sb_attention_e4m3_scratch_bytes(int n_rows, int n_q_heads, int
   return n <= 1 || n_rows <= 0 || n_q_heads <= 0 ? 0 : (size_t)n_rows * n_q_heads * n * PART * sizeof(float);
 }
 
-extern "C" int sb_attention_e4m3(const void* q, void* out, int n_rows, int n_seqs, int max_new, int max_len, const int32_t* seq_row0,
+extern "C" int sb_attention_e4m3(const void* q, void* out, int dtype, int n_rows, int n_seqs, int max_new, int max_len, const int32_t* seq_row0,
                                  const int32_t* seq_pos0, const int32_t* page_off, const int32_t* page_ids, int page_size,
                                  const void* cache, const float* scales, int n_pages, int n_q_heads, int n_kv_heads, int hd, int window,
                                  float scale, void* scratch, size_t scratch_bytes, cudaStream_t stream) {
@@ -532,25 +564,28 @@ extern "C" int sb_attention_e4m3(const void* q, void* out, int n_rows, int n_seq
   if (n_q_heads % n_kv_heads)
     SB_FAIL(SB_ERR_ARG, "%s: %d query heads are not a multiple of %d key/value heads", who, n_q_heads, n_kv_heads);
   if (window < 0) SB_FAIL(SB_ERR_ARG, "%s: window %d (0: none)", who, window);
-  if ((((uintptr_t)q | (uintptr_t)cache | (uintptr_t)scratch) & 15) || ((uintptr_t)out & 7)) SB_FAIL(SB_ERR_ARG, "%s: unaligned operands", who);
+  if ((((uintptr_t)q | (uintptr_t)cache | (uintptr_t)scratch) & 15) || ((uintptr_t)out & 15)) SB_FAIL(SB_ERR_ARG, "%s: unaligned operands", who);
+  if (!sb_valid_dtype(dtype)) SB_FAIL(SB_ERR_ARG, "%s: dtype code %d", who, dtype);
   const int G = n_q_heads / n_kv_heads, n_splits = most_splits(max_len);
   const long rows = (long)max_new * G;
-  const bool two = HD <= 128 && rows > 8;        // sixteen rows a block: the pages are read once for them
+  const bool two = HD <= 128 && dtype == SB_BF16 && rows > 8;     // sixteen rows a block: the pages are read once for them
   const long groups = (rows + (two ? 15 : 7)) / (two ? 16 : 8);
   if (groups * n_kv_heads > 65535 || n_seqs > 65535 || max_new > 65535 || n_splits > 8192)
     SB_FAIL(SB_ERR_UNSUPPORTED, "%s: %d new rows of %d/%d heads, %d sequences, max_len %d", who, max_new, n_q_heads, n_kv_heads, n_seqs, max_len);
   const size_t need = sb_attention_e4m3_scratch_bytes(n_rows, n_q_heads, max_len);
   if (need > scratch_bytes || (need && !scratch)) SB_FAIL(SB_ERR_ARG, "%s: %zu bytes of scratch needed, %zu given", who, need, scratch_bytes);
-  const Args a = {(const bf16*)q, (bf16*)out, seq_row0, seq_pos0, page_off, page_ids, (const uint8_t*)cache, scales, (float*)scratch,
+  const Args a = {q, out, seq_row0, seq_pos0, page_off, page_ids, (const uint8_t*)cache, scales, (float*)scratch,
                   n_q_heads, n_kv_heads, n_pages, window, n_splits, scale * LOG2E};
   const dim3 grid(n_splits, (unsigned)(groups * n_kv_heads), n_seqs);
 #if SB_HD <= 128
-  if (two) sb_launch<SB_K_ATTENTION>(attn_e4m3_kernel<2>, grid, dim3(WARPS * 32), 0, stream, a);
+  if (two) sb_launch<SB_K_ATTENTION>(attn_e4m3_kernel<2, bf16>, grid, dim3(WARPS * 32), 0, stream, a);
 #endif
-  if (!two) sb_launch<SB_K_ATTENTION>(attn_e4m3_kernel<1>, grid, dim3(WARPS * 32), 0, stream, a);
+  if (!two) SB_DISPATCH_DTYPE(dtype, T, { sb_launch<SB_K_ATTENTION>(attn_e4m3_kernel<1, T>, grid, dim3(WARPS * 32), 0, stream, a); });
   SB_CHECK_LAUNCH(who);
   if (n_splits > 1) {
-    sb_launch<SB_K_ATTENTION>(attn_e4m3_merge_kernel, dim3(n_q_heads, n_seqs, max_new), dim3(MERGE_THREADS), n_splits * sizeof(float), stream, a);
+    SB_DISPATCH_DTYPE(dtype, T, {
+      sb_launch<SB_K_ATTENTION>(attn_e4m3_merge_kernel<T>, dim3(n_q_heads, n_seqs, max_new), dim3(MERGE_THREADS), n_splits * sizeof(float), stream, a);
+    });
     SB_CHECK_LAUNCH(who);
   }
   return SB_OK;

@@ -20,6 +20,7 @@ __device__ __forceinline__ int own_page(const int32_t* page_off, const int32_t* 
 // scale is decided where all its new values are at hand, with no order between blocks.
 // Rotation of the pair (a, b): a c - b s, a s + b c, each product and sum rounded on its own, as everywhere in this library.
 constexpr int STORE_THREADS = 128;
+constexpr int STORE_FEW = 8;                      // new rows a sequence up to which a block's threads take one row a warp
 
 struct StoreArgs {
   const float *qkv, *angles;                     // [rows][(q heads + 2 kv heads) hd]; [rows][rot]: cosines, then sines
@@ -87,6 +88,129 @@ __global__ void __launch_bounds__(STORE_THREADS) store_kernel(const StoreArgs a)
   for (int pos = lo + warp; pos < hi; pos += STORE_THREADS / 32)
     for (int e = 2 * lane; e < a.hd; e += 64)
       *reinterpret_cast<uint16_t*>(dst + (size_t)(pos - start) * a.hd + e) = (uint16_t)to_e4m3x2(value(pos, e), value(pos, e + 1), inverse);
+}
+
+// The same for stretches of rows, for head sizes and rotated parts that are multiples of 8: a thread keeps eight values of up to P
+// rows in registers (four pairs four and four, or eight of the part beyond the rotation), so a value is read once, 16 bytes at a
+// time, between the rotation, the page's largest and the rounding; a block takes several heads, which share the rows' angles in
+// registers (as many as leave every SM blocks).
+constexpr int MANY_THREADS = 256;
+
+template <typename TQ>
+__device__ __forceinline__ void store_four(TQ* dst, const float* v);
+template <>
+__device__ __forceinline__ void store_four<float>(float* dst, const float* v) {
+  *reinterpret_cast<float4*>(dst) = make_float4(v[0], v[1], v[2], v[3]);
+}
+template <>
+__device__ __forceinline__ void store_four<__nv_bfloat16>(__nv_bfloat16* dst, const float* v) {
+  const __nv_bfloat162 x = __floats2bfloat162_rn(v[0], v[1]), y = __floats2bfloat162_rn(v[2], v[3]);
+  *reinterpret_cast<uint2*>(dst) = make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
+}
+__device__ __forceinline__ void load_four(float* v, const float* src) {
+  const float4 x = *reinterpret_cast<const float4*>(src);
+  v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
+}
+
+template <int P, typename TQ>
+__global__ void __launch_bounds__(MANY_THREADS) store_many_kernel(const StoreArgs a, int heads_per_block) {
+  __shared__ float warp_most[2][MANY_THREADS / 32];
+  sb_pdl_launch();
+  sb_pdl_wait();
+  const int seq = blockIdx.z, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int row0 = a.seq_row0[seq], n_new = a.seq_row0[seq + 1] - row0, pos0 = a.seq_pos0[seq];
+  if (n_new <= 0 || pos0 < 0) return;
+  const int nth = pos0 / a.page_size + blockIdx.x, start = nth * a.page_size;
+  const int lo = max(pos0, start), hi = min(pos0 + n_new, start + a.page_size);       // positions
+  if (lo >= hi) return;
+  const int page = own_page(a.page_off, a.page_ids, seq, nth, a.n_pages);
+  const int units = a.hd / 8, per_pass = MANY_THREADS / units, u = tid % units, r = tid / units;
+  const int half = a.rot >> 1, pairs = a.rot / 8, n_heads = a.n_q_heads + 2 * a.n_kv_heads, width = n_heads * a.hd;
+  const bool turns = u < pairs;
+  const int e1 = turns ? 4 * u : a.rot + 8 * (u - pairs), e2 = turns ? e1 + half : e1 + 4;
+  const int head0 = blockIdx.y * heads_per_block, head1 = min(head0 + heads_per_block, n_heads);
+  bool mine[P];
+  float cs[P][4], sn[P][4];
+#pragma unroll
+  for (int p = 0; p < P; ++p) {
+    const int at = r + p * per_pass;
+    mine[p] = r < per_pass && lo + at < hi;
+    if (mine[p] && turns && head0 < a.n_q_heads + a.n_kv_heads) {
+      const float* turn = a.angles + (size_t)(row0 + lo - pos0 + at) * a.rot + 4 * u;
+      load_four(cs[p], turn);
+      load_four(sn[p], turn + half);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) cs[p][i] = 1.0f, sn[p][i] = 0.0f;
+    }
+  }
+  for (int head = head0; head < head1; ++head) {
+    const bool is_q = head < a.n_q_heads, is_v = head >= a.n_q_heads + a.n_kv_heads;
+    if (!is_q && page < 0) return;               // no page of its own there: nothing is written
+    float x[P][8];
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[p][i] = 0.0f;
+      if (mine[p]) {
+        const float* src = a.qkv + (size_t)(row0 + lo - pos0 + r + p * per_pass) * width + (size_t)head * a.hd;
+        load_four(x[p], src + e1);
+        load_four(x[p] + 4, src + e2);
+      }
+    }
+    if (turns && !is_v) {
+#pragma unroll
+      for (int p = 0; p < P; ++p)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float y = x[p][i], z = x[p][4 + i];
+          x[p][i] = sb_rot_lo(y, z, cs[p][i], sn[p][i]);
+          x[p][4 + i] = sb_rot_hi(y, z, cs[p][i], sn[p][i]);
+        }
+    }
+    if (is_q) {
+#pragma unroll
+      for (int p = 0; p < P; ++p)
+        if (mine[p]) {
+          TQ* dst = (TQ*)a.q_out + ((size_t)(row0 + lo - pos0 + r + p * per_pass) * a.n_q_heads + head) * a.hd;
+          store_four<TQ>(dst + e1, x[p]);
+          store_four<TQ>(dst + e2, x[p] + 4);
+        }
+      continue;
+    }
+    const size_t block = (size_t)page * 2 * a.n_kv_heads + (head - a.n_q_heads);
+    uint8_t* dst = a.cache + block * a.page_size * a.hd;
+    const int before = lo > start ? exponent_of(a.scales[block]) : E4M3_LOWEST;        // of tokens of earlier steps
+    float most = 0.0f;
+#pragma unroll
+    for (int p = 0; p < P; ++p)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) most = fmaxf(most, e4m3_size(x[p][i]));
+    most = sb_warp_max(most);
+    float* shared = warp_most[head & 1];         // two of them: the next head's are written while these are read
+    if (lane == 0) shared[warp] = most;
+    __syncthreads();                             // and everybody has read the scale
+#pragma unroll
+    for (int w = 0; w < MANY_THREADS / 32; ++w) most = fmaxf(most, shared[w]);
+    const int need = e4m3_exponent(most), e = max(need, before);
+    if (lo > start && e > before) {
+      const float shrink = exp2f((float)(before - e));
+      for (int i = 4 * tid; i < (lo - start) * a.hd; i += 4 * MANY_THREADS) {
+        const uint32_t v = *reinterpret_cast<const uint32_t*>(dst + i);
+        const float2 y = e4m3x2_to_float2(v & 0xffffu), z = e4m3x2_to_float2(v >> 16);
+        *reinterpret_cast<uint32_t*>(dst + i) = to_e4m3x2(y.x, y.y, shrink) | to_e4m3x2(z.x, z.y, shrink) << 16;
+      }
+    }
+    if (tid == 0) a.scales[block] = exp2_int(e);
+    const float inverse = exp2_int(-e);
+#pragma unroll
+    for (int p = 0; p < P; ++p)
+      if (mine[p]) {
+        uint8_t* row = dst + (size_t)(lo - start + r + p * per_pass) * a.hd;
+        *reinterpret_cast<uint32_t*>(row + e1) = to_e4m3x2(x[p][0], x[p][1], inverse) | to_e4m3x2(x[p][2], x[p][3], inverse) << 16;
+        *reinterpret_cast<uint32_t*>(row + e2) = to_e4m3x2(x[p][4], x[p][5], inverse) | to_e4m3x2(x[p][6], x[p][7], inverse) << 16;
+      }
+  }
 }
 
 // -------------------------------------------------------------------------------------- values
@@ -225,7 +349,7 @@ attention_kernel(const TQ* q, TQ* out, const int32_t* row_seq, const int32_t* ro
 extern "C" int sb_rope_store_e4m3(const float* qkv, int n_rows, int n_seqs, int max_new, int n_q_heads, int n_kv_heads, int hd, int rot,
                                   const float* angles, const int32_t* seq_row0, const int32_t* seq_pos0, const int32_t* page_off,
                                   const int32_t* page_ids, int page_size, void* cache, float* scales, int n_pages, void* q_out, int q_dtype,
-                                  cudaStream_t stream) {
+                                  int n_sms, cudaStream_t stream) {
   const char* who = "sb_rope_store_e4m3";
   if (!qkv || !seq_row0 || !seq_pos0 || !page_off || !page_ids || !cache || !scales || !q_out) SB_FAIL(SB_ERR_ARG, "%s: an array is missing", who);
   if (n_rows <= 0 || n_seqs <= 0 || max_new <= 0 || n_q_heads <= 0 || n_kv_heads <= 0 || page_size <= 0 || n_pages <= 0)
@@ -239,7 +363,21 @@ extern "C" int sb_rope_store_e4m3(const float* qkv, int n_rows, int n_seqs, int 
     SB_FAIL(SB_ERR_UNSUPPORTED, "%s: %d sequences, %d/%d heads", who, n_seqs, n_q_heads, n_kv_heads);
   const StoreArgs a = {qkv, angles, seq_row0, seq_pos0, page_off, page_ids, (uint8_t*)cache, scales, q_out,
                        n_q_heads, n_kv_heads, hd, rot, page_size, n_pages};
-  const dim3 grid((unsigned)(((long)max_new + 2 * page_size - 2) / page_size), n_q_heads + 2 * n_kv_heads, n_seqs);
+  const int n_heads = n_q_heads + 2 * n_kv_heads;
+  dim3 grid((unsigned)(((long)max_new + 2 * page_size - 2) / page_size), n_heads, n_seqs);
+  const int passes = hd % 8 || hd > 8 * MANY_THREADS ? 99 : (page_size + MANY_THREADS / (hd / 8) - 1) / (MANY_THREADS / (hd / 8));
+  if (max_new > STORE_FEW && rot % 8 == 0 && passes <= 8 &&
+      (((uintptr_t)qkv | (uintptr_t)angles | (uintptr_t)q_out) & 15) == 0 && ((uintptr_t)cache & 3) == 0) {
+    const long blocks = (long)grid.x * n_heads * n_seqs, fill = blocks / (4L * (n_sms > 0 ? n_sms : 1));
+    const int per_block = (int)(fill < 1 ? 1 : fill > 8 ? 8 : fill);
+    grid.y = (n_heads + per_block - 1) / per_block;
+    SB_DISPATCH_DTYPE(q_dtype, TQ, {
+      sb_launch<SB_K_ELEMENTWISE>(passes <= 2 ? store_many_kernel<2, TQ> : passes <= 4 ? store_many_kernel<4, TQ> : store_many_kernel<8, TQ>, grid,
+                                  dim3(MANY_THREADS), 0, stream, a, per_block);
+    });
+    SB_CHECK_LAUNCH(who);
+    return SB_OK;
+  }
   SB_DISPATCH_DTYPE(q_dtype, TQ, { sb_launch<SB_K_ELEMENTWISE>(store_kernel<TQ>, grid, dim3(STORE_THREADS), 0, stream, a); });
   SB_CHECK_LAUNCH(who);
   return SB_OK;

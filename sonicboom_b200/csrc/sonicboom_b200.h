@@ -498,7 +498,7 @@ int sb_random_normal(void* out, int out_dtype, size_t n, uint32_t key0, uint32_t
 int sb_rope_store_e4m3(const float* qkv, int n_rows, int n_seqs, int max_new, int n_q_heads, int n_kv_heads, int hd, int rot,
                        const float* angles, const int32_t* seq_row0, const int32_t* seq_pos0, const int32_t* page_off,
                        const int32_t* page_ids, int page_size, void* cache, float* scales, int n_pages, void* q_out, int q_dtype,
-                       sb_stream_t stream);
+                       int n_sms, sb_stream_t stream);
 /* The pages of a step's sequences as values (exactly), one after another as page_ids [n_list] lists them, [k|v][kv head][position]
  * [hd] each, with the page list numbers [n_list] that says so; 0 at positions that no row of the step sees.  Pages wholly before the window are left out.  Sequences whose positions
  * have no pages get zeros in out [rows][n_q_heads * hd], of the values' dtype: what attends to the values leaves them alone. */
@@ -555,10 +555,10 @@ int sb_attention(const void* q, void* out, int n_rows, int n_seqs, int max_new,
                  size_t scratch_bytes, int* counters, int n_counters, int max_len, int n_pages,
                  int n_sms, const void* warm, size_t warm_bytes, const float* sink, float softcap,
                  int chunk, const float* bias, int bias_len, sb_stream_t stream);
-/* The same attention over a cache in 8 bits (see attn_e4m3.cu and sb_rope_store_e4m3), bfloat16 rows, pages of 64 keys; meant for
+/* The same attention over a cache in 8 bits (see attn_e4m3.cu and sb_rope_store_e4m3), rows of either type, pages of 64 keys; meant for
  * few rows a sequence.  scratch: sb_attention_e4m3_scratch_bytes of it.  Rows behind the last sequence are left as they are. */
 size_t sb_attention_e4m3_scratch_bytes(int n_rows, int n_q_heads, int max_len);
-int sb_attention_e4m3(const void* q, void* out, int n_rows, int n_seqs, int max_new, int max_len, const int32_t* seq_row0,
+int sb_attention_e4m3(const void* q, void* out, int dtype, int n_rows, int n_seqs, int max_new, int max_len, const int32_t* seq_row0,
                       const int32_t* seq_pos0, const int32_t* page_off, const int32_t* page_ids, int page_size, const void* cache,
                       const float* scales, int n_pages, int n_q_heads, int n_kv_heads, int hd, int window, float scale, void* scratch,
                       size_t scratch_bytes, sb_stream_t stream);

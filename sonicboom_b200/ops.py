@@ -711,11 +711,25 @@ def rope_store_e4m3(qkv: torch.Tensor, n_q_heads: int, n_kv_heads: int, head_dim
     _check(lib().sb_rope_store_e4m3(
         _ptr(qkv), n, plan.n_seqs, plan.max_new, n_q_heads, n_kv_heads, head_dim, rotary_dim, _ptr(angles),
         _i32(plan.seq_row0, "seq_row0"), _i32(plan.seq_pos0, "seq_pos0"), _i32(g.page_off, "page_off"), _i32(g.page_ids, "page_ids"),
-        g.page_size, _ptr(cache), _ptr(scales), cache.shape[0], _ptr(q_out), _code(q_out.dtype), _stream()), "rope_store_e4m3")
+        g.page_size, _ptr(cache), _ptr(scales), cache.shape[0], _ptr(q_out), _code(q_out.dtype),
+        _sm_count(qkv.device), _stream()), "rope_store_e4m3")
     return q_out
 
 
-E4M3_FEW_ROWS = 16               # rows (new tokens x heads) of one key/value head up to which pages are read as they are
+def _reads_pages_directly(plan, n_q_heads: int, n_kv_heads: int, head_dim: int, n_sms: int) -> bool:
+    """Whether bfloat16 rows attend to 8-bit pages as they are: sixteen rows of a key/value head at a time, the pages read and
+    converted again for every sixteen; or to their values, written out first, 256 rows at a time.  The first one's time grows with
+    rows x keys, the second one's with the keys that a block walks alone.  In us, fitted to 1 and 8 sequences, 7 to 448 rows, 100
+    to 16,000 keys, head sizes 64 and 128 (the choice is the faster one in all but near ties: 8 sequences of 112 rows over 900
+    keys 40 us and 28 us, 63 rows over 4,000 keys 64 us and 95 us, one of 448 rows over 4,000 keys 57 us and 77 us)."""
+    rows, keys = plan.max_new * (n_q_heads // n_kv_heads), plan.max_len
+    if rows <= 16:
+        return True
+    heads = plan.n_seqs * n_kv_heads
+    direct = 8.0 + (45 + 0.47 * head_dim) * 1e-6 * heads * ((rows + 15) // 16) * keys
+    blocks = heads * ((rows + 255) // 256)
+    values = 10.0 + 0.016 * keys * ((blocks + n_sms - 1) // n_sms) + 1.2e-6 * heads * head_dim * keys
+    return direct <= values
 
 
 class _ValuesPlan:
@@ -750,10 +764,10 @@ def attention_e4m3(q: torch.Tensor, out: torch.Tensor, plan, group_index: int, c
     n > 0 only the last n keys.  q and out bfloat16 or float32, of one dtype.  Rows behind the plan's last sequence are left as
     they are; a sequence whose positions have no pages gets zeros.
 
-    bfloat16 at head sizes in steps of 16 up to 256 and pages of 64 keys with few rows a sequence (up to E4M3_FEW_ROWS of a
-    key/value head) reads the pages on tensor cores.  More rows, and float32 at head sizes that are multiples of 4 up to 256, have
-    the step's pages brought to values first (exact, in the plan's scratch memory) and run `attention`.  Anything else, or
-    `kernel="plain"`, runs the plain kernel; `"few"` and `"values"` choose one of the others."""
+    Head sizes in steps of 16 up to 256 with pages of 64 keys run on tensor cores (built for the head size at first use): "few"
+    reads the pages as they are, float32 rows and weights as two halves each; bfloat16 rows in such numbers that this is slower
+    have the step's pages brought to values first (exact, in the plan's scratch memory) and run `attention`, and so does float32
+    at other head sizes that are multiples of 4 up to 256: "values".  Anything else runs the "plain" kernel.  `kernel` names one."""
     global LAUNCHES
     n, g = q.shape[0], plan.groups[group_index]
     _check_e4m3("attention_e4m3", plan, g, cache, scales, n_kv_heads, head_dim, n)
@@ -763,10 +777,10 @@ def attention_e4m3(q: torch.Tensor, out: torch.Tensor, plan, group_index: int, c
     aligned = (q.data_ptr() | cache.data_ptr() | out.data_ptr()) % 16 == 0
     few = values = False
     if kernel != "plain" and aligned:
-        few = q.dtype == torch.bfloat16 and head_dim in _build.HEAD_DIMS and g.page_size == 64
-        values = head_dim <= 256 and (few or (q.dtype == torch.float32 and head_dim % 4 == 0))
-        many = plan.max_new * (n_q_heads // n_kv_heads) > E4M3_FEW_ROWS
-        few = few and kernel != "values" and (kernel == "few" or not many)
+        few = head_dim in _build.HEAD_DIMS and g.page_size == 64
+        values = few or (q.dtype == torch.float32 and head_dim % 4 == 0 and head_dim <= 256)
+        few = few and kernel != "values" and (kernel == "few" or q.dtype == torch.float32 or _reads_pages_directly(
+            plan, n_q_heads, n_kv_heads, head_dim, _sm_count(q.device)))
     if kernel in ("few", "values") and not (few or values):
         raise KernelError(f"attention_e4m3: the kernel {kernel!r} does not take {q.dtype} at head size {head_dim}, pages of {g.page_size}")
     if values and not few:
@@ -775,7 +789,7 @@ def attention_e4m3(q: torch.Tensor, out: torch.Tensor, plan, group_index: int, c
     if al is not None:
         scratch = plan.scratch(int(al.sb_attention_e4m3_scratch_bytes(n, n_q_heads, plan.max_len)), q.device)
         rc = al.sb_attention_e4m3(
-            _ptr(q), _ptr(out), n, plan.n_seqs, plan.max_new, plan.max_len, _i32(plan.seq_row0, "seq_row0"),
+            _ptr(q), _ptr(out), _code(q.dtype), n, plan.n_seqs, plan.max_new, plan.max_len, _i32(plan.seq_row0, "seq_row0"),
             _i32(plan.seq_pos0, "seq_pos0"), _i32(g.page_off, "page_off"), _i32(g.page_ids, "page_ids"), g.page_size, _ptr(cache),
             _ptr(scales), cache.shape[0], n_q_heads, n_kv_heads, head_dim, window, ctypes.c_float(scale), _ptr(scratch),
             scratch.numel() if scratch is not None else 0, _stream())

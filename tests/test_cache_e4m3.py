@@ -43,7 +43,7 @@ def test_a_larger_scale_rounds_only_what_is_not_normal_any_more():
 def store(l, qkv=P, rows=4, seqs=2, max_new=2, hq=4, hkv=2, hd=64, rot=64, angles=P, row0=P, pos0=P, off=P, ids=P, page=64, cache=P,
           scales=P, pages=8, q=P, dtype=1):
     return l.sb_rope_store_e4m3(qkv, rows, seqs, max_new, hq, hkv, hd, rot, angles, row0, pos0, off, ids, page, cache, scales, pages, q, dtype,
-                                None)
+                                148, None)
 
 
 @pytest.mark.parametrize("kw,code", [

@@ -223,8 +223,7 @@ def test_attention_kernels_by_name(hd, kernel):
     """The same calls through every kernel, those "auto" would not choose among them."""
     attention_case([1, 3, 50], [70, 200, 20], 6, 2, hd, torch.bfloat16, kernel=kernel)
     attention_case([1, 3, 50], [70, 200, 20], 6, 2, hd, torch.bfloat16, kernel=kernel, window=33)
-    if kernel != "few":
-        attention_case([1, 3, 50], [70, 200, 20], 6, 2, hd, torch.float32, kernel=kernel)
+    attention_case([1, 3, 50], [70, 200, 20], 6, 2, hd, torch.float32, kernel=kernel)
 
 
 @pytest.mark.parametrize("new,pos0", [([1, 1, 1], [500, 39, 40]), ([2, 2], [300, 63]), ([90, 1, 64], [0, 200, 129])])
@@ -236,8 +235,9 @@ def test_attention_in_a_window(new, pos0, window, hd):
 
 @pytest.mark.parametrize("hq,hkv,hd", [(28, 4, 128), (6, 1, 64), (16, 1, 128), (17, 1, 128), (64, 2, 128)])
 @pytest.mark.parametrize("new", [1, 2, 3])
-def test_attention_of_few_rows_over_long_sequences(hq, hkv, hd, new):
-    attention_case([new, new, new], [5000, 4095, 2047 - new], hq, hkv, hd, torch.bfloat16, seed=new)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_attention_of_few_rows_over_long_sequences(hq, hkv, hd, new, dtype):
+    attention_case([new, new, new], [5000, 4095, 2047 - new], hq, hkv, hd, dtype, seed=new)
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
