@@ -119,6 +119,7 @@ ATTENTION = {
     "sb_attention_last_launches": ("i", ""),
     "sb_attention_scratch_bytes": ("z", "iiiii"),
     "sb_attention": ("i", "ppiiippppipiiiifpzpiiiipzpfipis"),
+    "sb_attention_e4m3_status": ("i", ""),
     "sb_attention_e4m3_scratch_bytes": ("z", "iii"),
     "sb_attention_e4m3": ("i", "ppiiiiippppippiiiiifpzs"),
     "sb_attention_decode_static": ("i", "ppiiippppipiiiifis"),

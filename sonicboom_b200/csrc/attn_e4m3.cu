@@ -3,15 +3,18 @@
 //
 //   out_i = sum_j exp2(s_ij - m) v_j / sum_j exp2(s_ij - m),   s_ij = scale log2(e) (q_i . k_j)
 //
-// over the keys j that row i sees.  What bounds it is reading every key and value byte once, so both go from global memory
-// straight into registers and through the tensor cores with the keys (and the value's dimensions) as the long side of the tile:
+// over the keys j that row i sees.  What bounds it is reading every key and value byte once; both go through the tensor cores with
+// the keys (and the value's dimensions) as the long side of the tile:
 //   S^T [16 keys x 8 rows] = K Q^T,   O^T [16 dims x 8 rows] += V^T P^T        (mma.sync m16n8k16, halves in, float32 out)
 // A tile's k index is a sum's order and nothing more, so a thread takes what lies together: 16 bytes of a key's row for four
-// k-steps of S, 16 bytes of each of four values' rows for eight tiles of O.  No shared memory, no barrier: a warp walks its
-// pages alone, with RING steps of 16 keys in flight.  e4m3 to half is exact.  q is brought to halves with a power of two for each
-// row: a bfloat16's 8 bits stay.  Weights are rounded to halves (2^-11) after they were summed in float32, times 2^15 so that
-// small ones stay normal numbers.  For float32 rows q and the weights are two halves each, the second what the first left over
-// (together within 2^-24 of a row's largest value, 2^-22 of a weight), and every product two.
+// k-steps of S, 16 bytes of each of four values' rows for eight tiles of O.  A warp walks its pages alone: one bulk copy brings a
+// page's keys of the head, another its values, into the warp's own shared memory, and the next page's are asked for as soon as
+// the tile has been read.  (Copies of 16 bytes a lane, into registers or shared memory, kept the memory at 4.4 of the 6.1 TB/s
+// that bulk copies of the same pages reach: 64 sequences of 512 to 8,192 keys 78 to 80 us instead of 62.)
+// e4m3 to half is exact.  q is brought to halves with a power of two for each row: a bfloat16's 8 bits stay.  Weights are rounded
+// to halves (2^-11) after they were summed in float32, times 2^15 so that small ones stay normal numbers.  For float32 rows q and
+// the weights are two halves each, the second what the first left over (together within 2^-24 of a row's largest value, 2^-22
+// of a weight), and every product two.
 //
 // Scales.  A page's key scale joins the score.  Its value scale 2^e joins the weight: with m the largest score so far and n the
 // largest of score + e, weights are exp2(s - m) in the sum and exp2(s + e - n) in the product with V, each at most 1, and
@@ -19,9 +22,12 @@
 //
 // A sequence's keys are cut into splits of whole pages by its own length alone, so a result depends on neither the batch nor
 // the pages' places: a block takes one split of one key/value head, warp w its pages w, w + 4, ..., merged in warp order; splits
-// are merged in ascending order by a second kernel.
+// are merged in ascending order by a second kernel.  (The block that is done last, by an arrival counter, took 3 us more than the
+// kernel's 2 at one sequence and as much more at 64; a cluster of the splits' blocks held shared memory for sequences with fewer
+// splits, 89 us instead of 62.)
 #include "common.cuh"
 #include "e4m3.cuh"
+#include "tc5.cuh"
 
 #ifndef SB_HD
 #define SB_HD 128
@@ -33,7 +39,8 @@ typedef __nv_bfloat16 bf16;
 constexpr int HD = SB_HD;
 constexpr int PAGE = 64;
 constexpr int WARPS = 4;
-constexpr int RING = HD > 128 ? 2 : 4;           // steps of 16 keys (or values) in flight a warp
+constexpr int TILE = PAGE * HD;                  // bytes of a page's keys, or values, of one head: one copy
+constexpr int AHEAD = HD > 64 ? 1 : HD > 32 ? 2 : 4;         // pages whose tiles a warp has room for
 constexpr int PART = HD + 4;                     // floats of a split's partial row: o, m, l
 constexpr float LOG2E = 1.4426950408889634f;
 // values of a thread: stretches of 128, 64, 32, 16 dims with 16, 8, 4, 2 bytes a lane, as head size has them
@@ -55,13 +62,19 @@ struct Args {
   float scale_log2;
 };
 
-// Pages of a split of a sequence of this length.
-__host__ __device__ constexpr int split_pages(int len) { return len <= 2048 ? 4 : len <= 8192 ? 8 : 16; }
-int most_splits(int max_len) {
-  int most = 1;
-  for (int len : {2048, 8192, max_len})
+// Pages of a split of a sequence of this length.  Shorter splits give few sequences enough blocks, longer ones cost many sequences
+// less (a block's start and its partial rows).  Four, eight and sixteen pages at 28/4 heads of 128, us with the merge: one sequence of
+// 1,500 keys 7.2, 9.2, 12.6 and 64 of them 32.7, 29.6, 30.9; of 6,000 keys 7.3, 9.0, 12.6 and 95.6, 77.3, 73.7; one of 30,000
+// 16.3, 14.3, 13.9 and four of them 34.9, 30.1, 26.7.
+__host__ __device__ constexpr int split_pages(int len) {
+  return len <= 2048 ? 4 : len <= 16384 ? 8 : len <= 131072 ? 16 : len <= 524288 ? 64 : 256;
+}
+constexpr int STRETCH = 8;                       // splits that are added up together
+long most_splits(int max_len) {
+  long most = 1;
+  for (long len : {2048L, 16384L, 131072L, 524288L, (long)max_len})
     if (len <= max_len) {
-      const int keys = split_pages(len) * PAGE, n = (len + keys - 1) / keys;
+      const long keys = split_pages((int)len) * PAGE, n = (len + keys - 1) / keys;
       if (n > most) most = n;
     }
   return most;
@@ -87,7 +100,7 @@ __device__ __forceinline__ Seq sequence(const Args& a, int b) {
 }
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
@@ -103,44 +116,43 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
 }
 
 template <int BYTES>
-__device__ __forceinline__ void load_bytes(uint32_t* dst, const uint8_t* src) {
+__device__ __forceinline__ void read_bytes(uint32_t* dst, const unsigned char* src) {
   if constexpr (BYTES == 16) {
-    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];\n" : "=r"(dst[0]), "=r"(dst[1]), "=r"(dst[2]), "=r"(dst[3]) : "l"(src));
+    const uint4 v = *reinterpret_cast<const uint4*>(src);
+    dst[0] = v.x; dst[1] = v.y; dst[2] = v.z; dst[3] = v.w;
   } else if constexpr (BYTES == 8) {
-    asm volatile("ld.global.L1::no_allocate.v2.u32 {%0,%1}, [%2];\n" : "=r"(dst[0]), "=r"(dst[1]) : "l"(src));
+    const uint2 v = *reinterpret_cast<const uint2*>(src);
+    dst[0] = v.x; dst[1] = v.y;
   } else if constexpr (BYTES == 4) {
-    asm volatile("ld.global.L1::no_allocate.u32 %0, [%1];\n" : "=r"(dst[0]) : "l"(src));
+    dst[0] = *reinterpret_cast<const uint32_t*>(src);
   } else {
-    uint16_t v;
-    asm volatile("ld.global.L1::no_allocate.u16 %0, [%1];\n" : "=h"(v) : "l"(src));
-    dst[0] = v;
+    dst[0] = *reinterpret_cast<const uint16_t*>(src);
   }
 }
 
-// Keys 16 sub + g and 16 sub + g + 8 of a page: thread t of a quad has bytes 16 t ... of every 64, 8 t ... of 32, 4 t ... of 16.
-__device__ __forceinline__ void load_keys(uint32_t (&w)[STEP_WORDS], const uint8_t* page, int sub, int g, int t) {
+// Keys 16 sub + g and 16 sub + g + 8 of a tile: thread t of a quad has bytes 16 t ... of every 64, 8 t ... of 32, 4 t ... of 16.
+__device__ __forceinline__ void read_keys(uint32_t (&w)[STEP_WORDS], const unsigned char* tile, int sub, int g, int t) {
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    const uint8_t* row = page + (size_t)(16 * sub + 8 * h + g) * HD;
+    const unsigned char* row = tile + (16 * sub + 8 * h + g) * HD;
     uint32_t* dst = w + h * K_WORDS;
-    int n = 0;
 #pragma unroll
-    for (int c = 0; c < HD / 64; ++c, n += 4) load_bytes<16>(dst + n, row + 64 * c + 16 * t);
-    if constexpr (N32) load_bytes<8>(dst + HD / 64 * 4, row + HD / 64 * 64 + 8 * t);
-    if constexpr (N16) load_bytes<4>(dst + HD / 64 * 4 + 2 * N32, row + HD / 64 * 64 + 32 * N32 + 4 * t);
+    for (int c = 0; c < HD / 64; ++c) read_bytes<16>(dst + 4 * c, row + 64 * c + 16 * t);
+    if constexpr (N32) read_bytes<8>(dst + HD / 64 * 4, row + HD / 64 * 64 + 8 * t);
+    if constexpr (N16) read_bytes<4>(dst + HD / 64 * 4 + 2 * N32, row + HD / 64 * 64 + 32 * N32 + 4 * t);
   }
 }
-// Values 16 sub + 2 t + {0, 1, 8, 9} of a page: lane g has bytes 16 g ... of every 128, 8 g ... of 64, and so on.
-__device__ __forceinline__ void load_values(uint32_t (&w)[STEP_WORDS], const uint8_t* page, int sub, int g, int t) {
+// Values 16 sub + 2 t + {0, 1, 8, 9} of a tile: lane g has bytes 16 g ... of every 128, 8 g ... of 64, and so on.
+__device__ __forceinline__ void read_values(uint32_t (&w)[STEP_WORDS], const unsigned char* tile, int sub, int g, int t) {
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const uint8_t* row = page + (size_t)(16 * sub + 2 * t + (j & 1) + 8 * (j >> 1)) * HD;
+    const unsigned char* row = tile + (16 * sub + 2 * t + (j & 1) + 8 * (j >> 1)) * HD;
     uint32_t* dst = w + j * V_WORDS;
 #pragma unroll
-    for (int c = 0; c < N128; ++c) load_bytes<16>(dst + 4 * c, row + 128 * c + 16 * g);
-    if constexpr (N64) load_bytes<8>(dst + 4 * N128, row + 128 * N128 + 8 * g);
-    if constexpr (N32) load_bytes<4>(dst + 4 * N128 + 2 * N64, row + 128 * N128 + 64 * N64 + 4 * g);
-    if constexpr (N16) load_bytes<2>(dst + 4 * N128 + 2 * N64 + N32, row + HD - 16 + 2 * g);
+    for (int c = 0; c < N128; ++c) read_bytes<16>(dst + 4 * c, row + 128 * c + 16 * g);
+    if constexpr (N64) read_bytes<8>(dst + 4 * N128, row + 128 * N128 + 8 * g);
+    if constexpr (N32) read_bytes<4>(dst + 4 * N128 + 2 * N64, row + 128 * N128 + 64 * N64 + 4 * g);
+    if constexpr (N16) read_bytes<2>(dst + 4 * N128 + 2 * N64 + N32, row + HD - 16 + 2 * g);
   }
 }
 // The dim of a thread's accumulator d, half h (rows g and g + 8 of tile d of O^T).
@@ -236,6 +248,12 @@ __device__ __forceinline__ void store_row(bf16* dst, float4 v) {
 }
 __device__ __forceinline__ void store_row(float* dst, float4 v) { *reinterpret_cast<float4*>(dst) = v; }
 
+__device__ __forceinline__ float exp2_approx(float x) {      // relative error 2^-22; 0 below 2^-126
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+  return y;
+}
+
 constexpr float WEIGHT_BITS = 15.0f;             // weights as halves are at most 2^15
 
 template <int NT, typename T>
@@ -243,11 +261,25 @@ __global__ void __launch_bounds__(WARPS * 32, HD <= 128 && NT == 1 && sizeof(T) 
   constexpr int ROWS = 8 * NT, PARTS = sizeof(T) / 2;
   const T* const q = (const T*)a.q;
   T* const out = (T*)a.out;
-  __shared__ __align__(16) float part[WARPS][ROWS][PART];
+  extern __shared__ __align__(128) unsigned char tiles[];           // [warp][AHEAD][k|v][TILE], then the warps' partial results
+  float(*part)[ROWS][PART] = reinterpret_cast<float(*)[ROWS][PART]>(tiles);
   __shared__ float stat_m[WARPS][ROWS], stat_l[WARPS][ROWS], stat_n[WARPS][ROWS];
+  __shared__ __align__(8) uint64_t landed[WARPS][2 * AHEAD];
+  __shared__ int failed;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  const unsigned char* const my_tiles = tiles + warp * (2 * AHEAD * TILE);
+  const uint32_t ring = (uint32_t)__cvta_generic_to_shared(my_tiles);
+  const uint32_t bars = (uint32_t)__cvta_generic_to_shared(landed[warp]);
+  if (tid == 0) failed = 0;
+  if (lane == 0) {                               // barriers and tiles of a warp's own
+#pragma unroll
+    for (int i = 0; i < 2 * AHEAD; ++i) mbar_init(bars + 8 * i, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+  }
+  __syncwarp();
   sb_pdl_wait();
   sb_pdl_launch();
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   const int split = blockIdx.x, kvh = blockIdx.y % a.n_kv_heads, row_base = blockIdx.y / a.n_kv_heads * ROWS, b = blockIdx.z;
   const int G = a.n_q_heads / a.n_kv_heads;
   const Seq sq = sequence(a, b);
@@ -261,6 +293,7 @@ __global__ void __launch_bounds__(WARPS * 32, HD <= 128 && NT == 1 && sizeof(T) 
     return;
   }
   if (split < sq.split_lo || split > sq.split_hi) return;
+  const bool single = sq.split_lo == sq.split_hi;
   // the rows' positions and what they see; the last row's lowest key and the first row's position bound the pages that all rows
   // see whole
   const int first_pos = sq.pos0 + row_base / G, last_pos = sq.pos0 + (min(row_base + ROWS, R) - 1) / G;
@@ -268,6 +301,29 @@ __global__ void __launch_bounds__(WARPS * 32, HD <= 128 && NT == 1 && sizeof(T) 
   const int low = low_of(first_pos), high_low = low_of(last_pos);
   const int tile_lo = max(split * sq.sp, low / PAGE), tile_hi = min(split * sq.sp + sq.sp - 1, last_pos / PAGE);
   const int32_t* pages = a.page_ids + a.page_off[b];
+  // Page i of this warp's (i from 0) goes to place i mod AHEAD; lane 0 asks for its tiles, every lane waits for them.
+  const int n_tiles = (tile_hi - tile_lo - warp + WARPS) / WARPS;   // none or less: no page is this warp's
+  const size_t kind = (size_t)a.n_kv_heads * TILE;
+  auto page_at = [&](int i) { return min(max(pages[tile_lo + warp + i * WARPS], 0), a.n_pages - 1); };
+  auto ask = [&](int i, int page, int v) {
+    const uint32_t place = 2 * (i % AHEAD) + v;
+    const uint8_t* src = a.cache + ((size_t)page * 2 * a.n_kv_heads + kvh) * TILE + v * kind;
+    mbar_expect_tx(bars + 8 * place, TILE);
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n" ::"r"(ring + place * TILE),
+                 "l"(src), "n"(TILE), "r"(bars + 8 * place) : "memory");
+  };
+  const size_t scale_stride = 2 * (size_t)a.n_kv_heads;
+  int page = n_tiles > 0 ? page_at(0) : 0;
+  if (lane == 0) {
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i)
+      if (i < n_tiles) {
+        const int p = i == 0 ? page : page_at(i);
+        ask(i, p, 0);
+        ask(i, p, 1);
+      }
+  }
+  float k_scale = a.scales[page * scale_stride + kvh], v_scale = a.scales[page * scale_stride + a.n_kv_heads + kvh];
 
   uint32_t qf[NT][HD / 16][2][PARTS];
   float fac[NT][2];                              // of rows 2t, 2t + 1: 2^x scale log2(e)
@@ -289,35 +345,37 @@ __global__ void __launch_bounds__(WARPS * 32, HD <= 128 && NT == 1 && sizeof(T) 
       for (int i = 0; i < 4; ++i) o[n][d][i] = 0.0f;
   }
 
-  const size_t kind = (size_t)a.n_kv_heads * PAGE * HD;
-  auto page_at = [&](int tile) { return min(max(pages[tile], 0), a.n_pages - 1); };
-  auto bytes_of = [&](int page) { return a.cache + ((size_t)page * 2 * a.n_kv_heads + kvh) * (PAGE * HD); };
-  uint32_t ring[RING][STEP_WORDS];
-  // step s = 0 ... 7 of a page: its keys in four steps, then its values
-  auto issue = [&](uint32_t (&w)[STEP_WORDS], const uint8_t* page, int s) {
-    if (s < 4) load_keys(w, page, s, g, t);
-    else load_values(w, page + kind, s - 4, g, t);
-  };
-  int tile = tile_lo + warp;
-  if (tile <= tile_hi) {
-    int page = page_at(tile);
-    const uint8_t* bytes = bytes_of(page);
+  // the rows' positions and first keys (a padding row sees nothing)
+  int row_pos[NT][2], row_low[NT][2];
 #pragma unroll
-    for (int s = 0; s < RING; ++s) issue(ring[s], bytes, s);
-    while (true) {
-      const float k_scale = a.scales[(size_t)page * 2 * a.n_kv_heads + kvh];
-      const int e = exponent_of(a.scales[((size_t)page * 2 + 1) * a.n_kv_heads + kvh]);
-      const bool more = tile + WARPS <= tile_hi;
-      const int next_page = more ? page_at(tile + WARPS) : page;
-      const uint8_t* next_bytes = bytes_of(next_page);
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const int row = row_base + 8 * n + 2 * t + r;
+      row_pos[n][r] = row < R ? sq.pos0 + row / G : -1;
+      row_low[n][r] = low_of(row_pos[n][r]);
+    }
+  int i = 0, gave_up = 0;                        // 1: at a page's keys, 2: at its values
+  for (; i < n_tiles; ++i) {
+    const uint32_t place = 2 * (i % AHEAD), parity = i / AHEAD & 1;
+    const int next = i + 1 < n_tiles ? page_at(i + 1) : page, ahead = i + AHEAD < n_tiles ? page_at(i + AHEAD) : 0;
+    const float next_k = a.scales[next * scale_stride + kvh], next_v = a.scales[next * scale_stride + a.n_kv_heads + kvh];
+    const int e = exponent_of(v_scale);
+    if (!__all_sync(0xffffffffu, mbar_wait(bars + 8 * place, parity, 31))) {
+      gave_up = 1;
+      break;
+    }
+    {
       float s[NT][4][4];
 #pragma unroll
       for (int sub = 0; sub < 4; ++sub) {
-        const uint32_t(&w)[STEP_WORDS] = ring[sub % RING];
+        uint32_t w[STEP_WORDS];
+        read_keys(w, my_tiles + place * TILE, sub, g, t);
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
           for (int i = 0; i < 4; ++i) s[n][sub][i] = 0.0f;
+        float s2[NT][4] = {};                    // every other step's sums: half as long a chain of products
 #pragma unroll
         for (int i = 0; i < HD / 16; ++i) {
           const uint32_t x = w[i], y = w[K_WORDS + i];
@@ -326,12 +384,16 @@ __global__ void __launch_bounds__(WARPS * 32, HD <= 128 && NT == 1 && sizeof(T) 
 #pragma unroll
           for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int j = 0; j < PARTS; ++j) mma_f16(s[n][sub], a0, a1, a2, a3, qf[n][i][0][j], qf[n][i][1][j]);
+            for (int j = 0; j < PARTS; ++j) mma_f16(i & 1 ? s2[n] : s[n][sub], a0, a1, a2, a3, qf[n][i][0][j], qf[n][i][1][j]);
         }
-        if (sub + RING < 8) issue(ring[sub % RING], bytes, sub + RING);
-        else if (more) issue(ring[sub % RING], next_bytes, sub + RING - 8);
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s[n][sub][i] += s2[n][i];
       }
-      const int key0 = tile * PAGE;
+      __syncwarp();
+      if (lane == 0 && i + AHEAD < n_tiles) ask(i + AHEAD, ahead, 0);
+      const int key0 = (tile_lo + warp + i * WARPS) * PAGE;
       const bool whole = key0 + PAGE - 1 <= first_pos && key0 >= high_low;      // every row sees every key
       uint32_t p[4][NT][2][PARTS];
 #pragma unroll
@@ -340,14 +402,16 @@ __global__ void __launch_bounds__(WARPS * 32, HD <= 128 && NT == 1 && sizeof(T) 
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
           const float f = fac[n][r] * k_scale;
-          const int row = row_base + 8 * n + 2 * t + r, pos = row < R ? sq.pos0 + row / G : -1, lo = low_of(pos);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            float& v = s[n][i >> 1][2 * (i & 1) + r];
-            const int key = key0 + 8 * i + g;
-            v = whole || (key <= pos && key >= lo) ? v * f : -INFINITY;
-            most[r] = fmaxf(most[r], v);
-          }
+          for (int j = 0; j < 8; ++j) s[n][j >> 1][2 * (j & 1) + r] *= f;
+          if (!whole)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              const int key = key0 + 8 * j + g;
+              if (key > row_pos[n][r] || key < row_low[n][r]) s[n][j >> 1][2 * (j & 1) + r] = -INFINITY;
+            }
+#pragma unroll
+          for (int j = 0; j < 8; ++j) most[r] = fmaxf(most[r], s[n][j >> 1][2 * (j & 1) + r]);
         }
         float shrink[2];
 #pragma unroll
@@ -356,14 +420,26 @@ __global__ void __launch_bounds__(WARPS * 32, HD <= 128 && NT == 1 && sizeof(T) 
           for (int x = 4; x < 32; x <<= 1) most[r] = fmaxf(most[r], __shfl_xor_sync(0xffffffffu, most[r], x));
           const float m_new = fmaxf(m[n][r], most[r]), ref_new = fmaxf(ref[n][r], most[r] + (float)e);
           const float m_at = m_new == -INFINITY ? 0.0f : m_new, ref_at = ref_new == -INFINITY ? 0.0f : ref_new;   // nothing seen: weights 0
-          l[n][r] *= exp2f(m[n][r] - m_at);
-          shrink[r] = exp2f(ref[n][r] - ref_at);
-          const float shift = (float)e - ref_at + WEIGHT_BITS;
+          l[n][r] *= exp2_approx(m[n][r] - m_at);
+          shrink[r] = exp2_approx(ref[n][r] - ref_at);
+          // exp2(s + e - n) as exp2(s - m) exp2(e + m - n), unless the references are so far apart that a factor leaves its range
+          const float apart = (float)e + m_at - ref_at;
+          if (__any_sync(0xffffffffu, fabsf(apart) > 64.0f)) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            float& v = s[n][i >> 1][2 * (i & 1) + r];
-            l[n][r] += exp2f(v - m_at);
-            v = exp2f(v + shift);
+            for (int j = 0; j < 8; ++j) {
+              float& v = s[n][j >> 1][2 * (j & 1) + r];
+              l[n][r] += exp2_approx(v - m_at);
+              v = exp2_approx(v + ((float)e - ref_at + WEIGHT_BITS));
+            }
+          } else {
+            const float factor = exp2_approx(apart + WEIGHT_BITS);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              float& v = s[n][j >> 1][2 * (j & 1) + r];
+              const float weight = exp2_approx(v - m_at);
+              l[n][r] += weight;
+              v = weight * factor;
+            }
           }
           m[n][r] = m_new;
           ref[n][r] = ref_new;
@@ -386,9 +462,14 @@ __global__ void __launch_bounds__(WARPS * 32, HD <= 128 && NT == 1 && sizeof(T) 
           }
         }
       }
+      if (!__all_sync(0xffffffffu, mbar_wait(bars + 8 * (place + 1), parity, 32))) {
+        gave_up = 2;
+        break;
+      }
 #pragma unroll
       for (int sub = 0; sub < 4; ++sub) {
-        uint32_t(&w)[STEP_WORDS] = ring[(sub + 4) % RING];
+        uint32_t w[STEP_WORDS];
+        read_values(w, my_tiles + (place + 1) * TILE, sub, g, t);
         if (!whole) {
           // Values that no row sees may hold anything, and 0 * NaN is NaN: they become 0.  A NaN that some rows see and others do
           // not goes to those that see it: it becomes 0 too, and a product of "is NaN" with "is seen" finds its rows.
@@ -433,17 +514,23 @@ __global__ void __launch_bounds__(WARPS * 32, HD <= 128 && NT == 1 && sizeof(T) 
           }
         }
         values_step<NT, PARTS>(o, w, p[sub]);
-        if (sub + 4 + RING < 8) issue(w, bytes, sub + 4 + RING);
-        else if (more) issue(w, next_bytes, sub + 4 + RING - 8);
       }
-      if (!more) break;
-      tile += WARPS;
-      page = next_page;
-      bytes = next_bytes;
+      __syncwarp();
+      if (lane == 0 && i + AHEAD < n_tiles) ask(i + AHEAD, ahead, 1);
     }
+    page = next;
+    k_scale = next_k;
+    v_scale = next_v;
+  }
+  if (gave_up) {                                 // nothing is written; the block's memory outlives its copies
+    for (int j = i; j < min(n_tiles, i + AHEAD + 1); ++j)
+      for (int v = 0; v < 2; ++v)
+        if (j < i + AHEAD || (v == 0 && gave_up == 2)) mbar_wait(bars + 8 * (2 * (j % AHEAD) + v), j / AHEAD & 1, 33);
+    failed = 1;
   }
 
-  // the warps' partial results
+  // the warps' partial results, over the tiles
+  __syncthreads();
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
 #pragma unroll
@@ -462,9 +549,10 @@ __global__ void __launch_bounds__(WARPS * 32, HD <= 128 && NT == 1 && sizeof(T) 
     }
   }
   __syncthreads();
-  const bool single = sq.split_lo == sq.split_hi;
-  for (int i = tid; i < min(ROWS, R - row_base) * (HD / 4); i += WARPS * 32) {
-    const int row = i / (HD / 4), c = 4 * (i % (HD / 4));
+  // merged in the warps' order: o relative to the largest score, that score, the weights' sum
+  const int n_items = failed ? 0 : min(ROWS, R - row_base) * (HD / 4);
+  for (int j = tid; j < n_items; j += WARPS * 32) {
+    const int row = j / (HD / 4), c = 4 * (j % (HD / 4));
     float mm = -INFINITY;
 #pragma unroll
     for (int w = 0; w < WARPS; ++w) mm = fmaxf(mm, stat_m[w][row]);
@@ -473,7 +561,7 @@ __global__ void __launch_bounds__(WARPS * 32, HD <= 128 && NT == 1 && sizeof(T) 
     float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
     for (int w = 0; w < WARPS; ++w) {
-      sum += stat_l[w][row] * exp2f(stat_m[w][row] - at);
+      sum += stat_l[w][row] * exp2_approx(stat_m[w][row] - at);
       const float f = exp2f(stat_n[w][row] - at);
       const float4 v = *reinterpret_cast<const float4*>(&part[w][row][c]);
       acc.x += v.x * f; acc.y += v.y * f; acc.z += v.z * f; acc.w += v.w * f;
@@ -490,70 +578,99 @@ __global__ void __launch_bounds__(WARPS * 32, HD <= 128 && NT == 1 && sizeof(T) 
   }
 }
 
-// Merges the splits of one row: weights from every split's maximum, then four groups of threads add a stretch of splits each in
-// ascending order, eight loads at a time, and the groups' sums are added in their order.  How the splits are shared out depends
-// on their number alone.
-constexpr int GROUPS = 4;
-constexpr int MERGE_THREADS = (HD / 4) * GROUPS;
+// Four values of a row over some splits: sum of weights times values and of weights, relative to the largest score m.
+struct Sum {
+  float4 v;
+  float m, l;
+};
+__device__ __forceinline__ void add(Sum& s, const Sum& x) {      // x, whose m is not above s.m
+  const float f = exp2_approx(x.m - (s.m == -INFINITY ? 0.0f : s.m));
+  s.v.x = fmaf(x.v.x, f, s.v.x); s.v.y = fmaf(x.v.y, f, s.v.y); s.v.z = fmaf(x.v.z, f, s.v.z); s.v.w = fmaf(x.v.w, f, s.v.w);
+  s.l = fmaf(x.l, f, s.l);
+}
+// The splits of a row are added up in stretches of STRETCH, in ascending order and with their loads issued together, then the
+// stretches in theirs: the same sums whoever forms them, so a row's bits depend on its sequence alone.
+__device__ __forceinline__ Sum sum_of_stretch(const float* row_splits, int i, int n_splits, int c) {
+  Sum x[STRETCH], s = {make_float4(0.0f, 0.0f, 0.0f, 0.0f), -INFINITY, 0.0f};
+#pragma unroll
+  for (int u = 0; u < STRETCH; ++u) {
+    const float* src = row_splits + (size_t)min(i * STRETCH + u, n_splits - 1) * PART;
+    x[u].v = __ldcg(reinterpret_cast<const float4*>(src + c));
+    const float2 ml = __ldcg(reinterpret_cast<const float2*>(src + HD));
+    x[u].m = ml.x;
+    x[u].l = ml.y;
+  }
+#pragma unroll
+  for (int u = 0; u < STRETCH; ++u)
+    if (i * STRETCH + u < n_splits) s.m = fmaxf(s.m, x[u].m);
+#pragma unroll
+  for (int u = 0; u < STRETCH; ++u)
+    if (i * STRETCH + u < n_splits) add(s, x[u]);
+  return s;
+}
+template <typename Stretch>
+__device__ __forceinline__ float4 joined(Stretch stretch, int n) {
+  Sum s = {make_float4(0.0f, 0.0f, 0.0f, 0.0f), -INFINITY, 0.0f};
+  for (int i = 0; i < n; ++i) s.m = fmaxf(s.m, stretch(i).m);
+  for (int i = 0; i < n; ++i) add(s, stretch(i));
+  const float inv = 1.0f / s.l;
+  return make_float4(s.v.x * inv, s.v.y * inv, s.v.z * inv, s.v.w * inv);
+}
+
+// Merges the splits of one row: a group of HD / 4 threads a stretch, as many groups as the longest sequence has stretches, up to
+// MOST_GROUPS (eight groups a block whatever the splits took 1,792 rows of at most eight splits 14 us instead of 5).  The kernel before this one lets
+// it start once it has waited itself, so the plan is there.  Dynamic shared memory: HD + 4 floats a stretch.
+constexpr int MOST_GROUPS = 8;
 template <typename T>
-__global__ void __launch_bounds__(MERGE_THREADS) attn_e4m3_merge_kernel(const Args a) {
-  extern __shared__ __align__(16) float weights[];                  // [n_splits]
-  __shared__ __align__(16) float sums[GROUPS][HD];
-  __shared__ float den[MERGE_THREADS];
-  sb_pdl_wait();
+__global__ void __launch_bounds__(HD / 4 * MOST_GROUPS) attn_e4m3_merge_kernel(const Args a) {
+  extern __shared__ __align__(16) float stretches[];                // [stretch][PART]: sums, then m and l
   sb_pdl_launch();
-  const int tid = threadIdx.x, head = blockIdx.x, b = blockIdx.y, row = blockIdx.z;
-  const Seq sq = sequence(a, b);
+  const int tid = threadIdx.x, head = blockIdx.x, row = blockIdx.z;
+  const Seq sq = sequence(a, blockIdx.y);
+  sb_pdl_wait();
   if (row >= sq.n_new || !sq.reads || sq.split_lo == sq.split_hi) return;
-  const int ns = sq.split_hi - sq.split_lo + 1;
+  const int ns = sq.split_hi - sq.split_lo + 1, n_stretches = (ns + STRETCH - 1) / STRETCH;
   const size_t at_row = (size_t)(sq.row0 + row) * a.n_q_heads + head;
   const float* src = a.scratch + (at_row * a.n_splits + sq.split_lo) * PART;
-  float mm = -INFINITY;
-  for (int i = tid; i < ns; i += MERGE_THREADS) {
-    const float v = __ldcg(src + (size_t)i * PART + HD);
-    weights[i] = v;
-    mm = fmaxf(mm, v);
+  const int c = 4 * (tid % (HD / 4));
+  for (int i = tid / (HD / 4); i < n_stretches; i += blockDim.x / (HD / 4)) {
+    const Sum s = sum_of_stretch(src, i, ns, c);
+    *reinterpret_cast<float4*>(stretches + (size_t)i * PART + c) = s.v;
+    if (c == 0) *reinterpret_cast<float2*>(stretches + (size_t)i * PART + HD) = make_float2(s.m, s.l);
   }
-  den[tid] = mm;
   __syncthreads();
-  for (int i = 0; i < MERGE_THREADS && i < ns; ++i) mm = fmaxf(mm, den[i]);
-  const float at = mm == -INFINITY ? 0.0f : mm;
-  __syncthreads();
-  for (int i = tid; i < ns; i += MERGE_THREADS) weights[i] = exp2f(weights[i] - at);
-  __syncthreads();
-  const int c = 4 * (tid % (HD / 4)), group = tid / (HD / 4), per = (ns + GROUPS - 1) / GROUPS;
-  float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  float sum = 0.0f;
-  for (int k = group * per; k < min(ns, (group + 1) * per); ++k) {
-    const float f = weights[k];
-    const float4 v = __ldcg(reinterpret_cast<const float4*>(src + (size_t)k * PART + c));
-    acc.x = fmaf(v.x, f, acc.x); acc.y = fmaf(v.y, f, acc.y); acc.z = fmaf(v.z, f, acc.z); acc.w = fmaf(v.w, f, acc.w);
-    sum = fmaf(__ldcg(src + (size_t)k * PART + HD + 1), f, sum);
-  }
-  *reinterpret_cast<float4*>(&sums[group][c]) = acc;
-  if (c == 0) den[group] = sum;
-  __syncthreads();
-  if (group) return;
-#pragma unroll
-  for (int i = 1; i < GROUPS; ++i) {
-    const float4 v = *reinterpret_cast<const float4*>(&sums[i][c]);
-    acc.x += v.x; acc.y += v.y; acc.z += v.z; acc.w += v.w;
-  }
-  const float inv = 1.0f / (((den[0] + den[1]) + den[2]) + den[3]);
-  store_row((T*)a.out + at_row * HD + c, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
+  if (tid >= HD / 4) return;
+  store_row((T*)a.out + at_row * HD + c, joined([&](int i) {
+    const float* s = stretches + (size_t)i * PART;
+    return Sum{*reinterpret_cast<const float4*>(s + c), s[HD], s[HD + 1]};
+  }, n_stretches));
 }
+
+template <int NT, typename T>
+cudaError_t launch(const Args& a, dim3 grid, cudaStream_t stream) {
+  constexpr int TILES = WARPS * 2 * AHEAD * TILE, PARTIALS = WARPS * 8 * NT * PART * 4, SMEM = TILES > PARTIALS ? TILES : PARTIALS;
+  if (cudaError_t e = sb_allow_shared<attn_e4m3_kernel<NT, T>>(SMEM)) return e;
+  return sb_launch<SB_K_ATTENTION>(attn_e4m3_kernel<NT, T>, grid, dim3(WARPS * 32), SMEM, stream, a);
+}
+
+// Blocks of a key/value head: sixteen rows each where they fit the registers (the pages are read once for them), else eight.
+bool sixteen_rows(int dtype, long rows) { return HD <= 128 && dtype == SB_BF16 && rows > 8; }
+long row_groups(int dtype, long rows) { return sixteen_rows(dtype, rows) ? (rows + 15) / 16 : (rows + 7) / 8; }
 
 }  // namespace
 
+// 0 when no kernel of this file has given up on a wait since the last call, else the code of that wait.
+extern "C" int sb_attention_e4m3_status() { return tc5_read_status(); }
+
 extern "C" size_t sb_attention_e4m3_scratch_bytes(int n_rows, int n_q_heads, int max_len) {
-  const int n = most_splits(max_len);
+  const long n = most_splits(max_len);
   return n <= 1 || n_rows <= 0 || n_q_heads <= 0 ? 0 : (size_t)n_rows * n_q_heads * n * PART * sizeof(float);
 }
 
-extern "C" int sb_attention_e4m3(const void* q, void* out, int dtype, int n_rows, int n_seqs, int max_new, int max_len, const int32_t* seq_row0,
-                                 const int32_t* seq_pos0, const int32_t* page_off, const int32_t* page_ids, int page_size,
-                                 const void* cache, const float* scales, int n_pages, int n_q_heads, int n_kv_heads, int hd, int window,
-                                 float scale, void* scratch, size_t scratch_bytes, cudaStream_t stream) {
+extern "C" int sb_attention_e4m3(const void* q, void* out, int dtype, int n_rows, int n_seqs, int max_new, int max_len,
+                                 const int32_t* seq_row0, const int32_t* seq_pos0, const int32_t* page_off, const int32_t* page_ids,
+                                 int page_size, const void* cache, const float* scales, int n_pages, int n_q_heads, int n_kv_heads, int hd,
+                                 int window, float scale, void* scratch, size_t scratch_bytes, cudaStream_t stream) {
   const char* who = "sb_attention_e4m3";
   if (hd != HD) SB_FAIL(SB_ERR_ARG, "%s: built for head size %d, called with %d", who, HD, hd);
   if (page_size != PAGE) SB_FAIL(SB_ERR_UNSUPPORTED, "%s: cache pages of %d keys (needs %d)", who, page_size, PAGE);
@@ -566,25 +683,28 @@ extern "C" int sb_attention_e4m3(const void* q, void* out, int dtype, int n_rows
   if (window < 0) SB_FAIL(SB_ERR_ARG, "%s: window %d (0: none)", who, window);
   if ((((uintptr_t)q | (uintptr_t)cache | (uintptr_t)scratch) & 15) || ((uintptr_t)out & 15)) SB_FAIL(SB_ERR_ARG, "%s: unaligned operands", who);
   if (!sb_valid_dtype(dtype)) SB_FAIL(SB_ERR_ARG, "%s: dtype code %d", who, dtype);
-  const int G = n_q_heads / n_kv_heads, n_splits = most_splits(max_len);
-  const long rows = (long)max_new * G;
-  const bool two = HD <= 128 && dtype == SB_BF16 && rows > 8;     // sixteen rows a block: the pages are read once for them
-  const long groups = (rows + (two ? 15 : 7)) / (two ? 16 : 8);
-  if (groups * n_kv_heads > 65535 || n_seqs > 65535 || max_new > 65535 || n_splits > 8192)
+  const long rows = (long)max_new * (n_q_heads / n_kv_heads), groups = row_groups(dtype, rows);
+  const long n_splits = most_splits(max_len), n_stretches = (n_splits + STRETCH - 1) / STRETCH;
+  if (groups * n_kv_heads > 65535 || n_seqs > 65535 || max_new > 65535 || n_stretches * PART * 4 > 48 * 1024)
     SB_FAIL(SB_ERR_UNSUPPORTED, "%s: %d new rows of %d/%d heads, %d sequences, max_len %d", who, max_new, n_q_heads, n_kv_heads, n_seqs, max_len);
   const size_t need = sb_attention_e4m3_scratch_bytes(n_rows, n_q_heads, max_len);
   if (need > scratch_bytes || (need && !scratch)) SB_FAIL(SB_ERR_ARG, "%s: %zu bytes of scratch needed, %zu given", who, need, scratch_bytes);
   const Args a = {q, out, seq_row0, seq_pos0, page_off, page_ids, (const uint8_t*)cache, scales, (float*)scratch,
-                  n_q_heads, n_kv_heads, n_pages, window, n_splits, scale * LOG2E};
-  const dim3 grid(n_splits, (unsigned)(groups * n_kv_heads), n_seqs);
+                  n_q_heads, n_kv_heads, n_pages, window, (int)n_splits, scale * LOG2E};
+  const dim3 grid((unsigned)n_splits, (unsigned)(groups * n_kv_heads), n_seqs);
+  cudaError_t e = cudaSuccess;
 #if SB_HD <= 128
-  if (two) sb_launch<SB_K_ATTENTION>(attn_e4m3_kernel<2, bf16>, grid, dim3(WARPS * 32), 0, stream, a);
+  if (sixteen_rows(dtype, rows)) e = launch<2, bf16>(a, grid, stream);
+  else
 #endif
-  if (!two) SB_DISPATCH_DTYPE(dtype, T, { sb_launch<SB_K_ATTENTION>(attn_e4m3_kernel<1, T>, grid, dim3(WARPS * 32), 0, stream, a); });
+    SB_DISPATCH_DTYPE(dtype, T, { e = launch<1, T>(a, grid, stream); });
+  if (e != cudaSuccess) SB_FAIL(SB_ERR_CUDA, "%s: %s", who, cudaGetErrorString(e));
   SB_CHECK_LAUNCH(who);
   if (n_splits > 1) {
+    const unsigned threads = HD / 4 * (unsigned)(n_stretches < MOST_GROUPS ? n_stretches : MOST_GROUPS);
     SB_DISPATCH_DTYPE(dtype, T, {
-      sb_launch<SB_K_ATTENTION>(attn_e4m3_merge_kernel<T>, dim3(n_q_heads, n_seqs, max_new), dim3(MERGE_THREADS), n_splits * sizeof(float), stream, a);
+      sb_launch<SB_K_ATTENTION>(attn_e4m3_merge_kernel<T>, dim3(n_q_heads, n_seqs, max_new), dim3(threads),
+                                n_stretches * PART * sizeof(float), stream, a);
     });
     SB_CHECK_LAUNCH(who);
   }

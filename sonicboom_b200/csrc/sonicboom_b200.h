@@ -555,8 +555,10 @@ int sb_attention(const void* q, void* out, int n_rows, int n_seqs, int max_new,
                  size_t scratch_bytes, int* counters, int n_counters, int max_len, int n_pages,
                  int n_sms, const void* warm, size_t warm_bytes, const float* sink, float softcap,
                  int chunk, const float* bias, int bias_len, sb_stream_t stream);
-/* The same attention over a cache in 8 bits (see attn_e4m3.cu and sb_rope_store_e4m3), rows of either type, pages of 64 keys; meant for
- * few rows a sequence.  scratch: sb_attention_e4m3_scratch_bytes of it.  Rows behind the last sequence are left as they are. */
+/* The same attention over a cache in 8 bits (see attn_e4m3.cu and sb_rope_store_e4m3), rows of either type, pages of 64 keys; meant
+ * for few rows a sequence.  scratch: sb_attention_e4m3_scratch_bytes of it; two calls that may run at the same time need
+ * scratch of their own.  Rows behind the last sequence are left as they are. */
+int sb_attention_e4m3_status(void);       /* as sb_tc5_status */
 size_t sb_attention_e4m3_scratch_bytes(int n_rows, int n_q_heads, int max_len);
 int sb_attention_e4m3(const void* q, void* out, int dtype, int n_rows, int n_seqs, int max_new, int max_len, const int32_t* seq_row0,
                       const int32_t* seq_pos0, const int32_t* page_off, const int32_t* page_ids, int page_size, const void* cache,

@@ -939,6 +939,10 @@ def check_status() -> None:
                 raise KernelError(f"the tensor-memory attention kernel of head size {hd} gave up "
                                   f"on a bounded wait (code {code}): results since the last check "
                                   "are incomplete")
+            code = int(l.sb_attention_e4m3_status())
+            if code > 0:
+                raise KernelError(f"the 8-bit attention kernel of head size {hd} gave up on a bounded wait (code {code}): "
+                                  "results since the last check are incomplete")
 
 
 def add_i32(x: torch.Tensor, delta: int) -> torch.Tensor:
