@@ -54,20 +54,34 @@ class StateNeed:
     dtype: torch.dtype = torch.float32
 
 
+E4M3 = torch.float8_e4m3fn       # the storage type of a cache in 8 bits
+
+
 class CacheGroup:
+    """With the dtype `E4M3` the storage holds 8-bit numbers and `scales` [entry, page, k|v, kv head] what they stand for (value =
+    number * scale; see `ops.rope_store_e4m3`); else there are no scales."""
+
     def __init__(self, need: KVNeed, entries: list[int], n_pages: int, page_size: int, dtype,
                  device):
         self.need, self.entries, self.page_size = need, list(entries), page_size
         self.pool = FreeList(n_pages, "page")
         # zeroed once: a page's unused tail is multiplied by zero probabilities, so it must
         # never hold NaN or infinity bit patterns; what sequences write later is finite
-        self.storage = torch.zeros((len(entries), n_pages, 2, need.n_kv_heads, page_size,
-                                    need.head_dim), dtype=dtype, device=device)
+        shape = (len(entries), n_pages, 2, need.n_kv_heads, page_size, need.head_dim)
+        if dtype == E4M3:
+            self.storage = torch.zeros(shape, dtype=torch.uint8, device=device).view(E4M3)
+            self.scales = torch.ones(shape[:4], dtype=torch.float32, device=device)
+        else:
+            self.storage, self.scales = torch.zeros(shape, dtype=dtype, device=device), None
         self._index = {e: i for i, e in enumerate(entries)}
 
     def entry_storage(self, entry: int) -> torch.Tensor:
         """[page, k|v, kv head, position in page, hd] of one schedule entry."""
         return self.storage[self._index[entry]]
+
+    def entry_scales(self, entry: int) -> Optional[torch.Tensor]:
+        """float32 [page, k|v, kv head] of one schedule entry of a cache in 8 bits; else None."""
+        return self.scales[self._index[entry]] if self.scales is not None else None
 
     def bytes_per_token(self) -> int:
         n = self.need
@@ -86,13 +100,13 @@ class Cache:
 
     def __init__(self, kv_needs: list, state_needs: list, max_tokens: int, dtype, device,
                  n_slots: Optional[int] = None, page_size: int = PAGE_SIZE,
-                 model_state: Optional[dict] = None):
+                 model_state: Optional[dict] = None, kv_dtype=None):
         """`kv_needs[i]` / `state_needs[i]` are what schedule entry i asks for (None: nothing; a
         state need is one StateNeed or a dict of them by name, the name None standing for the
         entry's unnamed one).  `model_state`: named StateNeeds
         that belong to no entry.
         `max_tokens` is the most tokens live sequences hold together, each sequence's count
-        rounded up to a whole page."""
+        rounded up to a whole page.  `kv_dtype`: the type keys and values are kept in, `dtype` when not given."""
         if max_tokens <= 0:
             raise CacheError(f"max_tokens = {max_tokens}")
         self.page_size = page_size
@@ -105,7 +119,7 @@ class Cache:
         for entry, need in enumerate(kv_needs):
             if need is not None:
                 by_need.setdefault(need, []).append(entry)
-        self.groups = [CacheGroup(need, entries, self.n_pages, page_size, dtype, device)
+        self.groups = [CacheGroup(need, entries, self.n_pages, page_size, kv_dtype or dtype, device)
                        for need, entries in by_need.items()]
         self.group_of_entry = {e: gi for gi, g in enumerate(self.groups) for e in g.entries}
         wanted = {}

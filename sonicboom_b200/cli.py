@@ -53,6 +53,7 @@ def main(argv=None) -> int:
     g.add_argument("--ctx", type=int, default=0,
                    help="cache size in tokens (default: what the prompts and -n need)")
     g.add_argument("--dtype", default="bfloat16", choices=["bfloat16", "float32"])
+    g.add_argument("--cache-dtype", default=None, choices=["e4m3"], help="keys and values in 8 bits (default: as --dtype)")
     g.add_argument("--device", default="cuda:0")
     g.add_argument("--ignore-eos", action="store_true", help="do not stop at the model's eos ids")
     g.add_argument("--stop", type=int, action="append", default=None, help="stop token id (repeatable)")
@@ -90,7 +91,8 @@ def main(argv=None) -> int:
                         presence_penalty=args.presence_penalty,
                         frequency_penalty=args.frequency_penalty)
     outs = llm.generate_batch(model, prompts, sampling=sampling, stop_tokens=args.stop,
-                              ignore_eos=args.ignore_eos, max_cache_tokens=args.ctx or None)
+                              ignore_eos=args.ignore_eos, max_cache_tokens=args.ctx or None,
+                              cache_dtype=args.cache_dtype)
     for ids in outs:
         print(" ".join(str(t) for t in ids))
     return 0

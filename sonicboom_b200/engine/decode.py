@@ -109,12 +109,22 @@ class DecodeLoop:
         # One eager run first: it builds what is built lazily and sets kernel attributes, which
         # cannot happen inside a capture.  It must leave the sequences as it found them: the
         # keys and values it writes at the current positions are overwritten by the first real
-        # step, and the slots' rows of every fixed-size state tensor are put back.
+        # step, and the slots' rows of every fixed-size state tensor are put back, and so are the
+        # pages at the current positions of a cache held in 8 bits, whose older numbers a new one may rescale.
         rows = self.plan.seq_slot.long()
         kept = {e: t[rows].clone() for e, t in cache.state.items()}
+        pages = []
+        for gi, g in enumerate(cache.groups):
+            if g.scales is not None:
+                ids = torch.tensor([cache.page_list(s, gi)[at // cache.page_size] for s, at in zip(self.slots, self.start)],
+                                   dtype=torch.int64, device=self.device)
+                for t in (g.storage.view(torch.uint8), g.scales):
+                    pages.append((t, ids, t[:, ids].clone()))
         self._one_step(advance=False)
         for e, t in cache.state.items():
             t[rows] = kept[e]
+        for t, ids, was in pages:
+            t[:, ids] = was
         self.launches_per_step = ops.LAUNCHES - before + 1
         torch.cuda.synchronize()
         ops.check_status()

@@ -57,12 +57,12 @@ class Session:
     per-token steps; the sampled draw is keyed by absolute position, so the same seed gives the
     same tokens however the calls are cut."""
 
-    def __init__(self, model: Model, n_ctx: int):
+    def __init__(self, model: Model, n_ctx: int, cache_dtype=None):
         if n_ctx <= 0:
             raise ValueError("n_ctx must be > 0")
         self.model = model
         self.n_ctx = min(int(n_ctx), model.decoder.spec.max_positions)
-        self.engine = Engine(model.decoder, max_tokens=self.n_ctx, n_slots=1)
+        self.engine = Engine(model.decoder, max_tokens=self.n_ctx, n_slots=1, cache_dtype=cache_dtype)
         self.sampler = Sampler(model.decoder.device)
         self.slot = None
         self.tokens: list = []          # prompt + everything decoded so far
@@ -157,9 +157,9 @@ class Session:
             self.slot = None
 
 
-def session_new(model: Model, n_ctx: int) -> Session:
-    """`boom_llm_session_new`."""
-    return Session(model, n_ctx)
+def session_new(model: Model, n_ctx: int, cache_dtype=None) -> Session:
+    """`boom_llm_session_new`.  `cache_dtype` "e4m3" keeps the session's keys and values in 8 bits (see `Engine`)."""
+    return Session(model, n_ctx, cache_dtype)
 
 
 def generate_tokens(session: Session, prompt, max_tokens: int, prefill: bool = True, *,
@@ -181,14 +181,15 @@ def generate_tokens(session: Session, prompt, max_tokens: int, prefill: bool = T
 def generate_batch(model: Model, prompts: list, max_tokens: int = 16, *, sampling=None,
                    stop_tokens=None, ignore_eos: bool = False, on_token=None,
                    max_cache_tokens: Optional[int] = None, max_batch: Optional[int] = None,
-                   engine: Optional[Engine] = None, **sampling_fields) -> list:
+                   engine: Optional[Engine] = None, cache_dtype=None, **sampling_fields) -> list:
     """Generates for many prompts (lists of token ids) at once.
 
     `sampling` is a Sampling (or one per prompt); without it one is made from `max_tokens`
     and the keyword fields (temperature, top_k, top_p, min_p, seed, repeat_penalty,
     repeat_last_n, presence_penalty, frequency_penalty).  Stop tokens default to the model's
     end-of-sequence ids unless `ignore_eos`.  The prompts run as one batch when the cache
-    holds them, else as several batches one after another."""
+    holds them, else as several batches one after another.  `cache_dtype` "e4m3" keeps keys and values in 8 bits (see `Engine`;
+    with an `engine` given, that one's cache is what it is)."""
     if sampling is None:
         sampling = Sampling(max_tokens=max_tokens, **sampling_fields)
     if stop_tokens is None:
@@ -198,6 +199,6 @@ def generate_batch(model: Model, prompts: list, max_tokens: int = 16, *, samplin
         need = sum((len(p) + (sampling.max_tokens if isinstance(sampling, Sampling)
                               else max(s.max_tokens for s in sampling)) + page - 1) // page * page
                    for p in prompts)
-        engine = Engine(model.decoder, max_tokens=min(need, max_cache_tokens or need))
+        engine = Engine(model.decoder, max_tokens=min(need, max_cache_tokens or need), cache_dtype=cache_dtype)
     return _generate(engine, Sampler(model.decoder.device), prompts, sampling, stop_tokens,
                      on_token, max_batch, model.decoder.spec.max_positions)

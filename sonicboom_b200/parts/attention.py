@@ -7,7 +7,7 @@ with scale applied after the dot and a causal (optionally windowed) mask
 spec may ask for one); the residual add is fused into that projection.  The three input projections are one product over a fused
 [q | k | v] matrix, the way the reference reads "sibling" weights in one launch
 (core/src/quant/mmvq_q8_1.cuh:634).  An entry that reads another entry's cache projects
-queries only."""
+queries only.  A cache held in 8 bits gets its rows from a kernel of its own behind the product."""
 from __future__ import annotations
 
 import torch
@@ -20,6 +20,8 @@ from .base import POSITION_ENCODINGS, Mixer, make, register_mixer
 
 @register_mixer("attention")
 class Attention(Mixer):
+    takes_e4m3 = True
+
     def __init__(self, spec, dtype, device):
         self.spec, self.dtype, self.device = spec, dtype, device
         self.hq, self.hkv, self.hd = spec.n_heads, spec.n_kv_heads, spec.head_dim
@@ -69,7 +71,11 @@ class Attention(Mixer):
         g = plan.groups[ctx.kv_group()]
         q = torch.empty((rows, self.hq, self.hd), dtype=self.dtype, device=h.device)
         w_in, rot = self.w_qkv[:width_in], self.position.rotary_dim
+        scales = ctx.kv_scales()
         angles = None
+        if scales is not None:
+            mixed = self._attend_e4m3(h, w_in, q, ctx, storage, scales)
+            return self._project(mixed, ctx, residual)
         if h.dtype == torch.bfloat16 and ops.takes_rotation_table(rows, w_in, self.hq, self.hkv, self.hd, rot, ctx.owns_cache):
             angles = ctx.rotation_table(self.position, self.spec.position)
         ops.qkv_rope_store(h, w_in,
@@ -80,8 +86,28 @@ class Attention(Mixer):
         mixed = torch.empty((rows, self.qw), dtype=self.dtype, device=h.device)
         ops.attention(q, mixed, plan, ctx.kv_group(), storage, self.hq, self.hkv, self.hd,
                       self.spec.window, self.spec.scale, warm=self.w_o)
+        return self._project(mixed, ctx, residual)
+
+    def _attend_e4m3(self, h, w_in, q, ctx, storage, scales):
+        """The rows' attention over a cache held in 8 bits."""
+        rows, plan, gi, rot = h.shape[0], ctx.plan, ctx.kv_group(), self.position.rotary_dim
+        bias = self.b_qkv[:w_in.shape[0]] if self.b_qkv is not None else None
+        if ctx.owns_cache:
+            qkv = torch.empty((rows, w_in.shape[0]), dtype=torch.float32, device=h.device)
+            ops.linear(h, w_in, qkv, ops.EPI_BIAS if bias is not None else ops.EPI_NONE, bias=bias)
+            angles = ctx.rotation_table(self.position, self.spec.position) if rot else None
+            ops.rope_store_e4m3(qkv, self.hq, self.hkv, self.hd, rot, angles, plan, gi, storage, scales, q)
+        else:
+            g = plan.groups[gi]
+            ops.qkv_rope_store(h, w_in, bias, self.hq, self.hkv, self.hd, rot, self.position.inv_freq, plan.row_seq, plan.row_pos,
+                               g.page_off, g.page_ids, g.page_size, None, q)
+        mixed = torch.empty((rows, self.qw), dtype=self.dtype, device=h.device)
+        return ops.attention_e4m3(q, mixed, plan, gi, storage, scales, self.hq, self.hkv, self.hd, self.spec.window, self.spec.scale)
+
+    def _project(self, mixed, ctx, residual):
+        rows = mixed.shape[0]
         out = residual if residual is not None else \
-            torch.empty((rows, self.spec.width), dtype=torch.float32, device=h.device)
+            torch.empty((rows, self.spec.width), dtype=torch.float32, device=mixed.device)
         epilogue = ops.EPI_RESIDUAL if residual is not None else ops.EPI_NONE
         if self.b_o is None:
             return ctx.linear(mixed, self.w_o, out, epilogue, residual=residual, act_dtype=self.dtype)

@@ -99,6 +99,11 @@ class StepContext:
         g = self.cache.groups[self.cache.group_of_entry[self.kv_entry]]
         return g.entry_storage(self.kv_entry)
 
+    def kv_scales(self) -> Optional[torch.Tensor]:
+        """[page, k|v, kv head] of that cache where it is held in 8 bits, else None."""
+        g = self.cache.groups[self.cache.group_of_entry[self.kv_entry]]
+        return g.entry_scales(self.kv_entry)
+
     def kv_group(self) -> int:
         return self.cache.group_of_entry[self.kv_entry]
 
@@ -153,6 +158,7 @@ class PositionEncoding(Part):
 class Mixer(Part):
     """forward(h [rows, width] in the activation dtype, ctx, residual=None) -> float32
     [rows, width]: the mixed rows, plus `residual` (which it may overwrite) when given."""
+    takes_e4m3 = False             # whether it writes and reads a cache held in 8 bits (`ctx.kv_scales()`)
 
     def kv_need(self) -> Optional[KVNeed]:
         return None

@@ -114,3 +114,39 @@ def test_tensors_that_are_not_on_a_gpu_are_refused():
     i = torch.zeros(2, dtype=torch.int32)
     with pytest.raises(ops.KernelError):
         ops.page_tables(i, i, i, torch.zeros(2, 4, dtype=torch.int32), i, i[:1], ops.PageTables(2, 4, 4, "cpu"), 1, 64)
+
+
+# ------------------------------------------------------------------------------------------------ cache and engine
+def test_cache_storage_and_scales():
+    from sonicboom_b200.cache import Cache, KVNeed
+    from sonicboom_b200.cache.kv import E4M3
+    c = Cache([KVNeed(2, 32), None, KVNeed(2, 32), KVNeed(1, 16, 40)], [None] * 4, 640, torch.bfloat16, "cpu", kv_dtype=E4M3)
+    assert [g.storage.dtype for g in c.groups] == [E4M3, E4M3]
+    assert c.groups[0].entry_storage(2).shape == (10, 2, 2, 64, 32) and c.groups[0].entry_scales(2).shape == (10, 2, 2)
+    assert c.groups[0].scales.dtype == torch.float32 and c.groups[0].bytes_per_token() == 2 * 2 * 2 * 32
+    plain_cache = Cache([KVNeed(2, 32)], [None], 640, torch.bfloat16, "cpu")
+    assert plain_cache.groups[0].scales is None and plain_cache.groups[0].entry_scales(0) is None
+    assert plain_cache.groups[0].storage.dtype == torch.bfloat16
+
+
+def test_engine_takes_it_for_plain_attention_only():
+    from conftest import TINY
+    from sonicboom_b200 import DecoderModel, Engine
+    from sonicboom_b200.cache.kv import E4M3
+    from sonicboom_b200.config import spec_from_config_dict
+    model = DecoderModel(spec_from_config_dict(TINY["C"])[1], torch.bfloat16, "cpu")
+    assert all(g.storage.dtype == E4M3 for g in Engine(model, 256, cache_dtype="e4m3").cache.groups)
+    assert all(g.storage.dtype == torch.bfloat16 for g in Engine(model, 256).cache.groups)
+    with pytest.raises(ValueError, match="cache_dtype"):
+        Engine(model, 256, cache_dtype="int8")
+    import zolulix_util
+    other = DecoderModel(spec_from_config_dict(next(iter(zolulix_util.CONFIGS.values())))[1], torch.bfloat16, "cpu")
+    with pytest.raises(ValueError, match="does not take"):
+        Engine(other, 256, cache_dtype="e4m3")
+
+
+def test_device_pages_refuse_sizes_without_room():
+    from sonicboom_b200.cache import CacheError, DevicePages
+    for sizes in ((0, 4, 4), (4, 0, 4), (4, 4, 0)):
+        with pytest.raises(CacheError):
+            DevicePages(*sizes, "cpu")
