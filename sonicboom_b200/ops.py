@@ -8,6 +8,7 @@ the kernel's own host-side checks, whose message is raised here.
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 
@@ -679,15 +680,26 @@ def _on_current_device(t, what) -> None:
         raise KernelError(f"{what}: tensors are on {t.device}, the current device is another: launches go to the current device's stream")
 
 
+def _plan_pointers(what, plan, g):
+    """Addresses of a plan's row and position offsets and of its page list, checked."""
+    row0, pos0, off, ids = arrays = plan.seq_row0, plan.seq_pos0, g.page_off, g.page_ids
+    if not row0.numel() == off.numel() == pos0.numel() + 1 == plan.n_seqs + 1:
+        raise KernelError(f"{what}: the plan's arrays are not those of {plan.n_seqs} sequences")
+    for t in arrays:
+        if t.dtype != torch.int32 or not t.is_cuda or not t.is_contiguous():
+            raise KernelError(f"{what}: a plan's arrays are contiguous int32 CUDA tensors")
+    return [t.data_ptr() for t in arrays]
+
+
 def _check_e4m3(what, plan, g, cache, scales, n_kv_heads, head_dim, n_rows) -> None:
     """What every kernel over an 8-bit cache asks of the plan and the cache."""
     _on_current_device(cache, what)
-    assert cache.dtype == E4M3 and cache.dim() == 5 and tuple(cache.shape[1:]) == (2, n_kv_heads, g.page_size, head_dim), \
-        f"{what}: cache is {cache.dtype} {tuple(cache.shape)}, want {E4M3} [pages, 2, {n_kv_heads}, {g.page_size}, {head_dim}]"
-    assert scales.dtype == torch.float32 and scales.shape == cache.shape[:3], \
-        f"{what}: scales are {scales.dtype} {tuple(scales.shape)}, want float32 {tuple(cache.shape[:3])}"
+    shape = cache.shape
+    assert cache.dtype == E4M3 and shape[1:] == (2, n_kv_heads, g.page_size, head_dim), \
+        f"{what}: cache is {cache.dtype} {tuple(shape)}, want {E4M3} [pages, 2, {n_kv_heads}, {g.page_size}, {head_dim}]"
+    assert scales.dtype == torch.float32 and scales.shape == shape[:3], \
+        f"{what}: scales are {scales.dtype} {tuple(scales.shape)}, want float32 {tuple(shape[:3])}"
     assert n_rows == plan.n_rows, f"{what}: {n_rows} rows, the plan has {plan.n_rows}"
-    assert plan.seq_row0.numel() == g.page_off.numel() == plan.n_seqs + 1 and plan.seq_pos0.numel() == plan.n_seqs
 
 
 def rope_store_e4m3(qkv: torch.Tensor, n_q_heads: int, n_kv_heads: int, head_dim: int, rotary_dim: int,
@@ -710,8 +722,7 @@ def rope_store_e4m3(qkv: torch.Tensor, n_q_heads: int, n_kv_heads: int, head_dim
         assert angles.dtype == torch.float32 and tuple(angles.shape) == (n, rotary_dim)
     _check(lib().sb_rope_store_e4m3(
         _ptr(qkv), n, plan.n_seqs, plan.max_new, n_q_heads, n_kv_heads, head_dim, rotary_dim, _ptr(angles),
-        _i32(plan.seq_row0, "seq_row0"), _i32(plan.seq_pos0, "seq_pos0"), _i32(g.page_off, "page_off"), _i32(g.page_ids, "page_ids"),
-        g.page_size, _ptr(cache), _ptr(scales), cache.shape[0], _ptr(q_out), _code(q_out.dtype),
+        *_plan_pointers("rope_store_e4m3", plan, g), g.page_size, _ptr(cache), _ptr(scales), cache.shape[0], _ptr(q_out), _code(q_out.dtype),
         _sm_count(qkv.device), _stream()), "rope_store_e4m3")
     return q_out
 
@@ -732,6 +743,11 @@ def _reads_pages_directly(plan, n_q_heads: int, n_kv_heads: int, head_dim: int, 
     return direct <= values
 
 
+@functools.lru_cache(maxsize=1024)
+def _e4m3_scratch_bytes(head_dim: int, n_rows: int, n_q_heads: int, max_len: int) -> int:
+    return int(attention_lib(head_dim).sb_attention_e4m3_scratch_bytes(n_rows, n_q_heads, max_len))
+
+
 class _ValuesPlan:
     """A plan whose pages lie one after another in scratch memory, for `attention`."""
 
@@ -750,9 +766,9 @@ def _attention_of_values(q, out, plan, g, cache, scales, n_q_heads, n_kv_heads, 
     nbytes = (n_list * cache[0].numel() * q.element_size() + 15) // 16 * 16
     scratch = plan.scratch(nbytes + 4 * n_list, q.device)
     values, numbers = scratch[:nbytes].view(q.dtype).view(n_list, *cache.shape[1:]), scratch[nbytes:nbytes + 4 * n_list].view(torch.int32)
+    row0, pos0, page_off, page_ids = _plan_pointers("attention_e4m3", plan, g)
     _check(lib().sb_cache_e4m3_values(
-        _i32(plan.seq_row0, "seq_row0"), _i32(plan.seq_pos0, "seq_pos0"), plan.n_seqs, plan.max_len, _i32(g.page_off, "page_off"),
-        _i32(g.page_ids, "page_ids"), n_list, g.page_size, _ptr(cache), _ptr(scales), cache.shape[0], n_q_heads, n_kv_heads, head_dim,
+        row0, pos0, plan.n_seqs, plan.max_len, page_off, page_ids, n_list, g.page_size, _ptr(cache), _ptr(scales), cache.shape[0], n_q_heads, n_kv_heads, head_dim,
         window, _ptr(values), _code(q.dtype), _ptr(numbers), _ptr(out), _stream()), "attention_e4m3 (values)")
     return attention(q, out, _ValuesPlan(plan, TableGroup(g.page_off, numbers, g.page_size)), 0, values, n_q_heads, n_kv_heads,
                      head_dim, window, scale)
@@ -777,21 +793,20 @@ def attention_e4m3(q: torch.Tensor, out: torch.Tensor, plan, group_index: int, c
     aligned = (q.data_ptr() | cache.data_ptr() | out.data_ptr()) % 16 == 0
     few = values = False
     if kernel != "plain" and aligned:
-        few = head_dim in _build.HEAD_DIMS and g.page_size == 64
+        few = head_dim % 16 == 0 and 16 <= head_dim <= 256 and g.page_size == 64
         values = few or (q.dtype == torch.float32 and head_dim % 4 == 0 and head_dim <= 256)
         few = few and kernel != "values" and (kernel == "few" or q.dtype == torch.float32 or _reads_pages_directly(
             plan, n_q_heads, n_kv_heads, head_dim, _sm_count(q.device)))
-    if kernel in ("few", "values") and not (few or values):
+    if kernel == "few" and not few or kernel == "values" and not values:
         raise KernelError(f"attention_e4m3: the kernel {kernel!r} does not take {q.dtype} at head size {head_dim}, pages of {g.page_size}")
     if values and not few:
         return _attention_of_values(q, out, plan, g, cache, scales, n_q_heads, n_kv_heads, head_dim, window, scale)
-    al = attention_lib(head_dim) if few else None
-    if al is not None:
-        scratch = plan.scratch(int(al.sb_attention_e4m3_scratch_bytes(n, n_q_heads, plan.max_len)), q.device)
+    if few:
+        al = attention_lib(head_dim)
+        scratch = plan.scratch(_e4m3_scratch_bytes(head_dim, n, n_q_heads, plan.max_len), q.device)
         rc = al.sb_attention_e4m3(
-            _ptr(q), _ptr(out), _code(q.dtype), n, plan.n_seqs, plan.max_new, plan.max_len, _i32(plan.seq_row0, "seq_row0"),
-            _i32(plan.seq_pos0, "seq_pos0"), _i32(g.page_off, "page_off"), _i32(g.page_ids, "page_ids"), g.page_size, _ptr(cache),
-            _ptr(scales), cache.shape[0], n_q_heads, n_kv_heads, head_dim, window, ctypes.c_float(scale), _ptr(scratch),
+            _ptr(q), _ptr(out), _code(q.dtype), n, plan.n_seqs, plan.max_new, plan.max_len, *_plan_pointers("attention_e4m3", plan, g),
+            g.page_size, _ptr(cache), _ptr(scales), cache.shape[0], n_q_heads, n_kv_heads, head_dim, window, scale, _ptr(scratch),
             scratch.numel() if scratch is not None else 0, _stream())
         if rc != 0:
             raise KernelError(f"attention_e4m3: {al.sb_last_error().decode()}")
@@ -864,12 +879,15 @@ def page_tables(slots: torch.Tensor, new: torch.Tensor, lengths: torch.Tensor, t
     same pages.  All arrays int32."""
     n = tables.n_seqs
     _on_current_device(lengths, "page_tables")
+    shape = table.shape
     assert slots.numel() == new.numel() == n, f"page_tables: {slots.numel()} slots, {new.numel()} counts, tables for {n} requests"
-    assert table.dim() == 2 and lengths.numel() == table.shape[0] and n_free.numel() == 1 and tables.device == lengths.device
+    assert len(shape) == 2 and lengths.numel() == shape[0] and n_free.numel() == 1 and tables.device == lengths.device
+    for t in (slots, new, lengths, table, free, n_free):
+        if t.dtype != torch.int32 or not t.is_cuda or not t.is_contiguous():
+            raise KernelError("page_tables: its arrays are contiguous int32 CUDA tensors")
     _check(lib().sb_page_tables(
-        _i32(slots, "slots"), _i32(new, "new"), n, _i32(lengths, "lengths"), _i32(table, "table"), table.shape[0], table.shape[1],
-        _i32(free, "free"), free.numel(), _i32(n_free, "n_free"), tables.page_size, tables.n_rows, tables.max_pages, max_new, max_len,
-        *tables._pointers, _stream()), "page_tables")
+        slots.data_ptr(), new.data_ptr(), n, lengths.data_ptr(), table.data_ptr(), *shape, free.data_ptr(), free.numel(), n_free.data_ptr(),
+        tables.page_size, tables.n_rows, tables.max_pages, max_new, max_len, *tables._pointers, _stream()), "page_tables")
     tables.max_new, tables.max_len = max_new, max_len
     return tables
 
