@@ -218,11 +218,31 @@ __global__ void __launch_bounds__(MANY_THREADS) store_many_kernel(const StoreArg
 // page_ids][k|v][head][position][hd], with `numbers` for the page list that says so.  Exact in either type (a number has four bits, the scale is a power of two).  What no row of
 // the step sees (positions behind a sequence's end, before its first row's window) becomes 0, whatever the page holds there; pages
 // that lie wholly before the window are left out.  A sequence whose positions have no pages gets rows of zeros in `out`, which
-// the attention behind this kernel leaves alone.  One block a page and head; bound by memory (1 byte in, 2 or 4 out a value).
-// It lets its successor start at its end only: that may read the plan ahead of its own wait.
+// the attention behind this kernel leaves alone.  One block a page and head, 16 bytes out a thread and step
+// (8 bytes in for bfloat16: with 16 in and 32 out a thread, 16,512 tokens took 24 us instead of 10); bound by memory (1 byte in, 2 or
+// 4 out a value) or, at few pages, by its start.  It lets its successor start at its end only: that may read `numbers` ahead of its own
+// wait, as attention of few rows does.
 constexpr int VALUES_THREADS = 128;
 
-template <typename T>
+// Numbers times a scale, 16 bytes of results: eight of bfloat16, four of float32 (or of bfloat16, 8 bytes).
+__device__ __forceinline__ uint32_t bf16_pair(uint32_t v, float scale) {
+  const float2 a = e4m3x2_to_float2(v);
+  const __nv_bfloat162 x = __floats2bfloat162_rn(a.x * scale, a.y * scale);
+  return *reinterpret_cast<const uint32_t*>(&x);
+}
+__device__ __forceinline__ void store_values(__nv_bfloat16* dst, const uint32_t (&v)[2], float scale) {
+  *reinterpret_cast<uint4*>(dst) = make_uint4(bf16_pair(v[0] & 0xffffu, scale), bf16_pair(v[0] >> 16, scale),
+                                              bf16_pair(v[1] & 0xffffu, scale), bf16_pair(v[1] >> 16, scale));
+}
+__device__ __forceinline__ void store_values(__nv_bfloat16* dst, const uint32_t (&v)[1], float scale) {
+  *reinterpret_cast<uint2*>(dst) = make_uint2(bf16_pair(v[0] & 0xffffu, scale), bf16_pair(v[0] >> 16, scale));
+}
+__device__ __forceinline__ void store_values(float* dst, const uint32_t (&v)[1], float scale) {
+  const float2 a = e4m3x2_to_float2(v[0] & 0xffffu), b = e4m3x2_to_float2(v[0] >> 16);
+  *reinterpret_cast<float4*>(dst) = make_float4(a.x * scale, a.y * scale, b.x * scale, b.y * scale);
+}
+
+template <int WORDS, typename T>
 __global__ void __launch_bounds__(VALUES_THREADS)
 values_kernel(const int32_t* seq_row0, const int32_t* seq_pos0, const int32_t* page_off, const int32_t* page_ids, int n_list, int page_size,
               const uint8_t* cache, const float* scales, int n_pages, int n_kv_heads, int hd, int window, T* values,
@@ -247,16 +267,27 @@ values_kernel(const int32_t* seq_row0, const int32_t* seq_pos0, const int32_t* p
   const uint32_t* src = reinterpret_cast<const uint32_t*>(cache + block * page_size * hd);
   T* dst = values + ((size_t)(first + i) * gridDim.y + head) * page_size * hd;
   const float scale = scales[block];
-#pragma unroll 4
-  for (int w = tid; w < page_size * hd / 4; w += VALUES_THREADS) {
-    const int pos = start + 4 * w / hd;
-    const uint32_t v = pos >= low && pos < len ? src[w] : 0;
-    const float2 a = e4m3x2_to_float2(v & 0xffffu), b = e4m3x2_to_float2(v >> 16);
-    if constexpr (sizeof(T) == 2) {
-      const __nv_bfloat162 x = __floats2bfloat162_rn(a.x * scale, a.y * scale), y = __floats2bfloat162_rn(b.x * scale, b.y * scale);
-      *reinterpret_cast<uint2*>(dst + 4 * (size_t)w) = make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
-    } else {
-      *reinterpret_cast<float4*>(dst + 4 * (size_t)w) = make_float4(a.x * scale, a.y * scale, b.x * scale, b.y * scale);
+  constexpr int STEPS = 8;                       // steps whose loads are issued together
+  for (int w0 = tid; w0 < page_size * hd / (4 * WORDS); w0 += STEPS * VALUES_THREADS) {
+    uint32_t v[STEPS][WORDS];
+#pragma unroll
+    for (int i = 0; i < STEPS; ++i) {
+      const int w = w0 + i * VALUES_THREADS, pos = start + 4 * WORDS * w / hd;
+#pragma unroll
+      for (int j = 0; j < WORDS; ++j) v[i][j] = 0;
+      if (w >= page_size * hd / (4 * WORDS) || pos < low || pos >= len) continue;
+      if constexpr (WORDS == 2) {
+        const uint2 x = *reinterpret_cast<const uint2*>(src + 2 * (size_t)w);
+        v[i][0] = x.x; v[i][1] = x.y;
+      } else {
+        v[i][0] = src[w];
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < STEPS; ++i) {
+      const int w = w0 + i * VALUES_THREADS;
+      if (w >= page_size * hd / (4 * WORDS)) break;
+      store_values(dst + 4 * WORDS * (size_t)w, v[i], scale);
     }
   }
 }
@@ -399,7 +430,11 @@ extern "C" int sb_cache_e4m3_values(const int32_t* seq_row0, const int32_t* seq_
   if (n_seqs > 65535 || n_kv_heads > 32767) SB_FAIL(SB_ERR_UNSUPPORTED, "%s: %d sequences, %d key/value heads", who, n_seqs, n_kv_heads);
   const dim3 grid((max_len + page_size - 1) / page_size, 2 * n_kv_heads, n_seqs);
   SB_DISPATCH_DTYPE(dtype, T, {
-    sb_launch<SB_K_ELEMENTWISE>(values_kernel<T>, grid, dim3(VALUES_THREADS), 0, stream, seq_row0, seq_pos0, page_off, page_ids, n_list,
+    auto kernel = values_kernel<1, T>;
+    if constexpr (sizeof(T) == 2) {
+      if (hd % 8 == 0) kernel = values_kernel<2, T>;
+    }
+    sb_launch<SB_K_ELEMENTWISE>(kernel, grid, dim3(VALUES_THREADS), 0, stream, seq_row0, seq_pos0, page_off, page_ids, n_list,
                                 page_size, (const uint8_t*)cache, scales, n_pages, n_kv_heads, hd, window, (T*)values, numbers, (T*)out,
                                 n_q_heads * hd);
   });
