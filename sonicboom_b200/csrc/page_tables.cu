@@ -17,7 +17,7 @@
 namespace {
 
 constexpr int TB = 512;                          // threads
-constexpr int CHUNK = 4 * TB;                    // rows or pages that a block fills in one go
+constexpr int CHUNK = 2 * TB;                    // rows or pages that a block fills in one go
 constexpr int MAX_SEQS = 8192;                   // five numbers of every request in shared memory
 constexpr int MAX_SLOTS = 1 << 18;               // a bit of every slot in shared memory
 constexpr int MAX_COUNT = 1 << 21;               // rows, pages of a slot: sums of a tile of requests stay inside 32 bits
@@ -62,6 +62,7 @@ __global__ void __launch_bounds__(TB) page_tables_kernel(const TableArgs a) {
   for (int i = tid; i < (a.n_slots + 31) / 32; i += TB) seen[i] = 0;
   if (tid == 0) found = 0;
   sb_pdl_wait();
+  const int n_free = a.n_free[0];
   __syncthreads();
   long long rows = 0, pages = 0, needed = 0;     // of the tiles before this one
   for (int first = 0; first < a.n_seqs; first += TB) {
@@ -109,7 +110,6 @@ __global__ void __launch_bounds__(TB) page_tables_kernel(const TableArgs a) {
     rows += tile.rows; pages += tile.total; needed += tile.taken;
     __syncthreads();
   }
-  const int n_free = a.n_free[0];
   int status = found;
   if (rows > a.max_rows) status |= SB_TABLES_ROWS;
   if (pages > a.max_pages) status |= SB_TABLES_PAGE_LIST;
@@ -274,7 +274,7 @@ extern "C" int sb_page_tables(const int32_t* slots, const int32_t* fresh, int n_
     SB_FAIL(SB_ERR_CUDA, "%s: shared memory opt-in failed: %s", who, cudaGetErrorString(e));
   const size_t smem = ((size_t)5 * n_seqs + 2 + (n_slots + 31) / 32) * 4;
   const long chunks = (max_rows + CHUNK - 1) / CHUNK + ((long)max_pages + CHUNK - 1) / CHUNK;
-  sb_launch<SB_K_OTHER>(page_tables_kernel, dim3((unsigned)(chunks < 128 ? chunks : 128)), dim3(TB), smem, stream, a);
+  sb_launch<SB_K_OTHER>(page_tables_kernel, dim3((unsigned)(chunks < 256 ? chunks : 256)), dim3(TB), smem, stream, a);
   SB_CHECK_LAUNCH(who);
   return SB_OK;
 }
