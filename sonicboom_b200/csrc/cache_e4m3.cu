@@ -20,7 +20,7 @@ __device__ __forceinline__ int own_page(const int32_t* page_off, const int32_t* 
 // scale is decided where all its new values are at hand, with no order between blocks.
 // Rotation of the pair (a, b): a c - b s, a s + b c, each product and sum rounded on its own, as everywhere in this library.
 constexpr int STORE_THREADS = 128;
-constexpr int STORE_FEW = 8;                      // new rows a sequence up to which a block's threads take one row a warp
+constexpr int STORE_FEW = 8;                      // new rows a sequence up to which a warp takes a head
 
 struct StoreArgs {
   const float *qkv, *angles;                     // [rows][(q heads + 2 kv heads) hd]; [rows][rot]: cosines, then sines
@@ -90,10 +90,11 @@ __global__ void __launch_bounds__(STORE_THREADS) store_kernel(const StoreArgs a)
       *reinterpret_cast<uint16_t*>(dst + (size_t)(pos - start) * a.hd + e) = (uint16_t)to_e4m3x2(value(pos, e), value(pos, e + 1), inverse);
 }
 
-// The same for stretches of rows, for head sizes and rotated parts that are multiples of 8: a thread keeps eight values of up to P
-// rows in registers (four pairs four and four, or eight of the part beyond the rotation), so a value is read once, 16 bytes at a
-// time, between the rotation, the page's largest and the rounding; a block takes several heads, which share the rows' angles in
-// registers (as many as leave every SM blocks).
+// The same for head sizes and rotated parts that are multiples of 8: a thread keeps eight values of up to P rows in registers (four
+// pairs four and four, or eight of the part beyond the rotation), so a value is read once, 16 bytes at a time, between the rotation,
+// the page's largest and the rounding.  Stretches of rows: 256 threads, several heads a block, which share the rows' angles in
+// registers (as many as leave every SM blocks); 2,048 rows of 28/4 heads of 128 14 us, 8.5 at the memory's pace, where a warp a row
+// with every value read twice took 47.  Up to STORE_FEW rows: a warp a head.
 constexpr int MANY_THREADS = 256;
 
 template <typename TQ>
@@ -112,9 +113,9 @@ __device__ __forceinline__ void load_four(float* v, const float* src) {
   v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
 }
 
-template <int P, typename TQ>
-__global__ void __launch_bounds__(MANY_THREADS) store_many_kernel(const StoreArgs a, int heads_per_block) {
-  __shared__ float warp_most[2][MANY_THREADS / 32];
+template <int THREADS, int P, typename TQ>
+__global__ void __launch_bounds__(THREADS) store_many_kernel(const StoreArgs a, int heads_per_block) {
+  __shared__ float warp_most[2][THREADS / 32];
   sb_pdl_launch();
   sb_pdl_wait();
   const int seq = blockIdx.z, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -124,7 +125,7 @@ __global__ void __launch_bounds__(MANY_THREADS) store_many_kernel(const StoreArg
   const int lo = max(pos0, start), hi = min(pos0 + n_new, start + a.page_size);       // positions
   if (lo >= hi) return;
   const int page = own_page(a.page_off, a.page_ids, seq, nth, a.n_pages);
-  const int units = a.hd / 8, per_pass = MANY_THREADS / units, u = tid % units, r = tid / units;
+  const int units = a.hd / 8, per_pass = THREADS / units, u = tid % units, r = tid / units;
   const int half = a.rot >> 1, pairs = a.rot / 8, n_heads = a.n_q_heads + 2 * a.n_kv_heads, width = n_heads * a.hd;
   const bool turns = u < pairs;
   const int e1 = turns ? 4 * u : a.rot + 8 * (u - pairs), e2 = turns ? e1 + half : e1 + 4;
@@ -191,11 +192,11 @@ __global__ void __launch_bounds__(MANY_THREADS) store_many_kernel(const StoreArg
     if (lane == 0) shared[warp] = most;
     __syncthreads();                             // and everybody has read the scale
 #pragma unroll
-    for (int w = 0; w < MANY_THREADS / 32; ++w) most = fmaxf(most, shared[w]);
+    for (int w = 0; w < THREADS / 32; ++w) most = fmaxf(most, shared[w]);
     const int need = e4m3_exponent(most), e = max(need, before);
     if (lo > start && e > before) {
       const float shrink = exp2f((float)(before - e));
-      for (int i = 4 * tid; i < (lo - start) * a.hd; i += 4 * MANY_THREADS) {
+      for (int i = 4 * tid; i < (lo - start) * a.hd; i += 4 * THREADS) {
         const uint32_t v = *reinterpret_cast<const uint32_t*>(dst + i);
         const float2 y = e4m3x2_to_float2(v & 0xffffu), z = e4m3x2_to_float2(v >> 16);
         *reinterpret_cast<uint32_t*>(dst + i) = to_e4m3x2(y.x, y.y, shrink) | to_e4m3x2(z.x, z.y, shrink) << 16;
@@ -396,18 +397,23 @@ extern "C" int sb_rope_store_e4m3(const float* qkv, int n_rows, int n_seqs, int 
                        n_q_heads, n_kv_heads, hd, rot, page_size, n_pages};
   const int n_heads = n_q_heads + 2 * n_kv_heads;
   dim3 grid((unsigned)(((long)max_new + 2 * page_size - 2) / page_size), n_heads, n_seqs);
-  const int passes = hd % 8 || hd > 8 * MANY_THREADS ? 99 : (page_size + MANY_THREADS / (hd / 8) - 1) / (MANY_THREADS / (hd / 8));
-  if (max_new > STORE_FEW && rot % 8 == 0 && passes <= 8 &&
+  if (hd % 8 == 0 && rot % 8 == 0 && hd <= 8 * MANY_THREADS &&
       (((uintptr_t)qkv | (uintptr_t)angles | (uintptr_t)q_out) & 15) == 0 && ((uintptr_t)cache & 3) == 0) {
+    const bool few = max_new <= STORE_FEW && hd <= 256;
+    const int per_pass = (few ? 32 : MANY_THREADS) / (hd / 8), rows = few ? max_new : page_size, passes = (rows + per_pass - 1) / per_pass;
     const long blocks = (long)grid.x * n_heads * n_seqs, fill = blocks / (4L * (n_sms > 0 ? n_sms : 1));
-    const int per_block = (int)(fill < 1 ? 1 : fill > 8 ? 8 : fill);
-    grid.y = (n_heads + per_block - 1) / per_block;
-    SB_DISPATCH_DTYPE(q_dtype, TQ, {
-      sb_launch<SB_K_ELEMENTWISE>(passes <= 2 ? store_many_kernel<2, TQ> : passes <= 4 ? store_many_kernel<4, TQ> : store_many_kernel<8, TQ>, grid,
-                                  dim3(MANY_THREADS), 0, stream, a, per_block);
-    });
-    SB_CHECK_LAUNCH(who);
-    return SB_OK;
+    const int per_block = few ? 1 : (int)(fill < 1 ? 1 : fill > 8 ? 8 : fill);
+    if (passes <= 8) {
+      grid.y = (n_heads + per_block - 1) / per_block;
+      SB_DISPATCH_DTYPE(q_dtype, TQ, {
+        auto kernel = few ? (passes <= 1 ? store_many_kernel<32, 1, TQ> : passes <= 4 ? store_many_kernel<32, 4, TQ> : store_many_kernel<32, 8, TQ>)
+                          : passes <= 2 ? store_many_kernel<MANY_THREADS, 2, TQ>
+                                        : passes <= 4 ? store_many_kernel<MANY_THREADS, 4, TQ> : store_many_kernel<MANY_THREADS, 8, TQ>;
+        sb_launch<SB_K_ELEMENTWISE>(kernel, grid, dim3(few ? 32 : MANY_THREADS), 0, stream, a, per_block);
+      });
+      SB_CHECK_LAUNCH(who);
+      return SB_OK;
+    }
   }
   SB_DISPATCH_DTYPE(q_dtype, TQ, { sb_launch<SB_K_ELEMENTWISE>(store_kernel<TQ>, grid, dim3(STORE_THREADS), 0, stream, a); });
   SB_CHECK_LAUNCH(who);

@@ -72,6 +72,7 @@ def rows_of(n, hq, hkv, hd, g, size=1.0):
 STEPS = [  # what every sequence brings, step by step: first tokens, page ends, single tokens, nothing, several pages
     [[1, 64, 5, 0, 130], [1, 1, 59, 3, 0], [62, 0, 1, 61, 1], [1, 129, 64, 1, 70]],
     [[333], [1], [1], [50], [1]],
+    [[3, 8, 1, 0], [5, 2, 8, 1], [60, 62, 50, 70], [1, 2, 3, 4], [8, 8, 8, 8]],
 ]
 
 
