@@ -674,32 +674,52 @@ def attention_status(head_dim: int) -> int:
 E4M3 = torch.float8_e4m3fn
 
 
-def _on_current_device(t, what) -> None:
-    index = t.device.index
-    if t.is_cuda and index != (_raw_device() if _raw_device is not None else torch.cuda.current_device()):
-        raise KernelError(f"{what}: tensors are on {t.device}, the current device is another: launches go to the current device's stream")
+_I32T, _F32T = torch.int32, torch.float32
 
 
-def _plan_pointers(what, plan, g):
-    """Addresses of a plan's row and position offsets and of its page list, checked."""
+def _device_of(t, what) -> int:
+    """The index of a tensor's device, which has to be the current one: launches go to the current device's stream."""
+    index = t.get_device()
+    if index < 0:
+        raise KernelError("kernels take CUDA tensors only; there is no CPU path")
+    if index != (_raw_device() if _raw_device is not None else torch.cuda.current_device()):
+        raise KernelError(f"{what}: tensors are on {t.device}, the current device is another")
+    return index
+
+
+def _stream_of(index: int):
+    return _raw_stream(index) if _raw_stream is not None else torch.cuda.current_stream().cuda_stream
+
+
+def _addresses(what, index, *tensors):
+    """The addresses of contiguous tensors on one device."""
+    found = []
+    for t in tensors:
+        if t.get_device() != index or not t.is_contiguous():
+            raise KernelError(f"{what}: kernels take contiguous tensors on one device, got one of shape {tuple(t.shape)} on {t.device}, "
+                              f"want cuda:{index}")
+        found.append(t.data_ptr())
+    return found
+
+
+def _check_plan(what, plan, g):
+    """The arrays of a plan that kernels over an 8-bit cache read: row and position offsets, a group's page list."""
     row0, pos0, off, ids = arrays = plan.seq_row0, plan.seq_pos0, g.page_off, g.page_ids
     if not row0.numel() == off.numel() == pos0.numel() + 1 == plan.n_seqs + 1:
         raise KernelError(f"{what}: the plan's arrays are not those of {plan.n_seqs} sequences")
-    for t in arrays:
-        if t.dtype != torch.int32 or not t.is_cuda or not t.is_contiguous():
-            raise KernelError(f"{what}: a plan's arrays are contiguous int32 CUDA tensors")
-    return [t.data_ptr() for t in arrays]
+    if row0.dtype is not _I32T or pos0.dtype is not _I32T or off.dtype is not _I32T or ids.dtype is not _I32T:
+        raise KernelError(f"{what}: a plan's arrays are int32")
+    return arrays
 
 
-def _check_e4m3(what, plan, g, cache, scales, n_kv_heads, head_dim, n_rows) -> None:
-    """What every kernel over an 8-bit cache asks of the plan and the cache."""
-    _on_current_device(cache, what)
+def _check_cache(what, cache, scales, g, n_kv_heads, head_dim):
     shape = cache.shape
-    assert cache.dtype == E4M3 and shape[1:] == (2, n_kv_heads, g.page_size, head_dim), \
-        f"{what}: cache is {cache.dtype} {tuple(shape)}, want {E4M3} [pages, 2, {n_kv_heads}, {g.page_size}, {head_dim}]"
-    assert scales.dtype == torch.float32 and scales.shape == shape[:3], \
-        f"{what}: scales are {scales.dtype} {tuple(scales.shape)}, want float32 {tuple(shape[:3])}"
-    assert n_rows == plan.n_rows, f"{what}: {n_rows} rows, the plan has {plan.n_rows}"
+    if n_kv_heads <= 0:
+        raise KernelError(f"{what}: {n_kv_heads} key/value heads")
+    if cache.dtype is not E4M3 or shape[1:] != (2, n_kv_heads, g.page_size, head_dim):
+        raise KernelError(f"{what}: cache is {cache.dtype} {tuple(shape)}, want {E4M3} [pages, 2, {n_kv_heads}, {g.page_size}, {head_dim}]")
+    if scales.dtype is not _F32T or scales.shape != shape[:3]:
+        raise KernelError(f"{what}: scales are {scales.dtype} {tuple(scales.shape)}, want float32 {tuple(shape[:3])}")
 
 
 def rope_store_e4m3(qkv: torch.Tensor, n_q_heads: int, n_kv_heads: int, head_dim: int, rotary_dim: int,
@@ -714,28 +734,38 @@ def rope_store_e4m3(qkv: torch.Tensor, n_q_heads: int, n_kv_heads: int, head_dim
     count for it and are stored as NaN.  A page that holds tokens of earlier steps keeps them: where the new ones need a larger
     scale its older numbers go over to it, which rounds only what falls below e4m3's normal numbers.  A page's first token starts
     its scale anew.  Rows behind the plan's last sequence are left as they are."""
-    n, g = qkv.shape[0], plan.groups[group_index]
-    _check_e4m3("rope_store_e4m3", plan, g, cache, scales, n_kv_heads, head_dim, n)
-    assert qkv.dtype == torch.float32 and qkv.dim() == 2 and qkv.shape[1] == (n_q_heads + 2 * n_kv_heads) * head_dim
-    assert q_out.numel() == n * n_q_heads * head_dim
+    what, n, g = "rope_store_e4m3", plan.n_rows, plan.groups[group_index]
+    index = _device_of(qkv, what)
+    _check_cache(what, cache, scales, g, n_kv_heads, head_dim)
+    if qkv.dtype is not _F32T or qkv.shape != (n, (n_q_heads + 2 * n_kv_heads) * head_dim):
+        raise KernelError(f"{what}: rows are {qkv.dtype} {tuple(qkv.shape)}, want float32 [{n}, {(n_q_heads + 2 * n_kv_heads) * head_dim}]")
+    if q_out.numel() != n * n_q_heads * head_dim:
+        raise KernelError(f"{what}: q_out is {tuple(q_out.shape)}, want [{n}, {n_q_heads}, {head_dim}]")
+    turn = None
     if angles is not None:
-        assert angles.dtype == torch.float32 and tuple(angles.shape) == (n, rotary_dim)
+        if angles.dtype is not _F32T or angles.shape != (n, rotary_dim):
+            raise KernelError(f"{what}: angles are {angles.dtype} {tuple(angles.shape)}, want float32 [{n}, {rotary_dim}]")
+        (turn,) = _addresses(what, index, angles)
+    rows, kept, kept_scales, q, row0, pos0, off, ids = _addresses(what, index, qkv, cache, scales, q_out, *_check_plan(what, plan, g))
     _check(lib().sb_rope_store_e4m3(
-        _ptr(qkv), n, plan.n_seqs, plan.max_new, n_q_heads, n_kv_heads, head_dim, rotary_dim, _ptr(angles),
-        *_plan_pointers("rope_store_e4m3", plan, g), g.page_size, _ptr(cache), _ptr(scales), cache.shape[0], _ptr(q_out), _code(q_out.dtype),
-        _sm_count(qkv.device), _stream()), "rope_store_e4m3")
+        rows, n, plan.n_seqs, plan.max_new, n_q_heads, n_kv_heads, head_dim, rotary_dim, turn, row0, pos0, off, ids, g.page_size, kept,
+        kept_scales, cache.shape[0], q, _code(q_out.dtype), _sm_count(index), _stream_of(index)), what)
     return q_out
 
 
-def _reads_pages_directly(plan, n_q_heads: int, n_kv_heads: int, head_dim: int, n_sms: int) -> bool:
-    """Whether bfloat16 rows attend to 8-bit pages as they are: sixteen rows of a key/value head at a time, the pages read and
+def _reads_pages_directly(plan, dtype, n_q_heads: int, n_kv_heads: int, head_dim: int, n_sms: int) -> bool:
+    """Whether rows attend to 8-bit pages as they are: sixteen bfloat16 rows of a key/value head at a time, the pages read and
     converted again for every sixteen; or to their values, written out first, 256 rows at a time.  The first one's time grows with
     rows x keys, the second one's with the keys that a block walks alone.  In us, fitted to 1 and 8 sequences, 7 to 448 rows, 100
     to 16,000 keys, head sizes 64 and 128 (the choice is the faster one in all but near ties: 8 sequences of 112 rows over 900
-    keys 40 us and 28 us, 63 rows over 4,000 keys 64 us and 95 us, one of 448 rows over 4,000 keys 57 us and 77 us)."""
+    keys 40 us and 28 us, 63 rows over 4,000 keys 64 us and 95 us, one of 448 rows over 4,000 keys 57 us and 77 us).
+    float32 rows do, eight at a time, as far as a grid and a few GB of partial rows go: their other way is 2.5 to 40 times slower."""
     rows, keys = plan.max_new * (n_q_heads // n_kv_heads), plan.max_len
     if rows <= 16:
         return True
+    if dtype is _F32T:
+        return plan.max_new <= 65535 and (rows + 7) // 8 * n_kv_heads <= 65535 and \
+            _e4m3_scratch_bytes(head_dim, plan.n_rows, n_q_heads, keys) <= 4 << 30
     heads = plan.n_seqs * n_kv_heads
     direct = 8.0 + (45 + 0.47 * head_dim) * 1e-6 * heads * ((rows + 15) // 16) * keys
     blocks = heads * ((rows + 255) // 256)
@@ -760,16 +790,16 @@ class _ValuesPlan:
         return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes > 0 else None
 
 
-def _attention_of_values(q, out, plan, g, cache, scales, n_q_heads, n_kv_heads, head_dim, window, scale):
+def _attention_of_values(q, out, plan, g, cache, scales, n_q_heads, n_kv_heads, head_dim, window, scale, index):
     """`attention_e4m3` by way of the step's pages as values of q's type."""
-    n_list = g.page_ids.numel()
+    what, n_list = "attention_e4m3", g.page_ids.numel()
     nbytes = (n_list * cache[0].numel() * q.element_size() + 15) // 16 * 16
     scratch = plan.scratch(nbytes + 4 * n_list, q.device)
-    values, numbers = scratch[:nbytes].view(q.dtype).view(n_list, *cache.shape[1:]), scratch[nbytes:nbytes + 4 * n_list].view(torch.int32)
-    row0, pos0, page_off, page_ids = _plan_pointers("attention_e4m3", plan, g)
+    values, numbers = scratch[:nbytes].view(q.dtype).view(n_list, *cache.shape[1:]), scratch[nbytes:nbytes + 4 * n_list].view(_I32T)
+    kept, kept_scales, to, listed, rows, row0, pos0, off, ids = _addresses(what, index, cache, scales, values, numbers, out, *_check_plan(what, plan, g))
     _check(lib().sb_cache_e4m3_values(
-        row0, pos0, plan.n_seqs, plan.max_len, page_off, page_ids, n_list, g.page_size, _ptr(cache), _ptr(scales), cache.shape[0], n_q_heads, n_kv_heads, head_dim,
-        window, _ptr(values), _code(q.dtype), _ptr(numbers), _ptr(out), _stream()), "attention_e4m3 (values)")
+        row0, pos0, plan.n_seqs, plan.max_len, off, ids, n_list, g.page_size, kept, kept_scales, cache.shape[0], n_q_heads, n_kv_heads,
+        head_dim, window, to, _code(q.dtype), listed, rows, _stream_of(index)), "attention_e4m3 (values)")
     return attention(q, out, _ValuesPlan(plan, TableGroup(g.page_off, numbers, g.page_size)), 0, values, n_q_heads, n_kv_heads,
                      head_dim, window, scale)
 
@@ -785,37 +815,42 @@ def attention_e4m3(q: torch.Tensor, out: torch.Tensor, plan, group_index: int, c
     have the step's pages brought to values first (exact, in the plan's scratch memory) and run `attention`, and so does float32
     at other head sizes that are multiples of 4 up to 256: "values".  Anything else runs the "plain" kernel.  `kernel` names one."""
     global LAUNCHES
-    n, g = q.shape[0], plan.groups[group_index]
-    _check_e4m3("attention_e4m3", plan, g, cache, scales, n_kv_heads, head_dim, n)
-    assert q.dtype == out.dtype and q.numel() == out.numel() == n * n_q_heads * head_dim
+    what, n, g, dtype = "attention_e4m3", plan.n_rows, plan.groups[group_index], q.dtype
+    index = _device_of(q, what)
+    _check_cache(what, cache, scales, g, n_kv_heads, head_dim)
+    if dtype is not out.dtype or not q.numel() == out.numel() == n * n_q_heads * head_dim or q.shape[0] != n:
+        raise KernelError(f"{what}: q is {dtype} {tuple(q.shape)}, out {out.dtype} {tuple(out.shape)}, want one type and [{n}, {n_q_heads}, {head_dim}]")
     if kernel not in ("auto", "plain", "few", "values"):
-        raise KernelError(f"attention_e4m3: unknown kernel {kernel!r}")
-    aligned = (q.data_ptr() | cache.data_ptr() | out.data_ptr()) % 16 == 0
+        raise KernelError(f"{what}: unknown kernel {kernel!r}")
+    if n_q_heads % n_kv_heads:
+        raise KernelError(f"{what}: {n_q_heads} query heads are not a multiple of {n_kv_heads} key/value heads")
     few = values = False
-    if kernel != "plain" and aligned:
+    rows, to, kept, kept_scales, row0, pos0, off, ids = _addresses(what, index, q, out, cache, scales, *_check_plan(what, plan, g))
+    if to == rows:
+        raise KernelError(f"{what}: q and out share memory: a row's query is read by several blocks until the last one is done")
+    if kernel != "plain" and (rows | to | kept) % 16 == 0:
         few = head_dim % 16 == 0 and 16 <= head_dim <= 256 and g.page_size == 64
-        values = few or (q.dtype == torch.float32 and head_dim % 4 == 0 and head_dim <= 256)
-        few = few and kernel != "values" and (kernel == "few" or q.dtype == torch.float32 or _reads_pages_directly(
-            plan, n_q_heads, n_kv_heads, head_dim, _sm_count(q.device)))
+        values = few or (dtype is _F32T and head_dim % 4 == 0 and head_dim <= 256)
+        few = few and kernel != "values" and (kernel == "few" or _reads_pages_directly(
+            plan, dtype, n_q_heads, n_kv_heads, head_dim, _sm_count(index)))
     if kernel == "few" and not few or kernel == "values" and not values:
-        raise KernelError(f"attention_e4m3: the kernel {kernel!r} does not take {q.dtype} at head size {head_dim}, pages of {g.page_size}")
-    if values and not few:
-        return _attention_of_values(q, out, plan, g, cache, scales, n_q_heads, n_kv_heads, head_dim, window, scale)
+        raise KernelError(f"{what}: the kernel {kernel!r} does not take {dtype} at head size {head_dim}, pages of {g.page_size}")
     if few:
         al = attention_lib(head_dim)
         scratch = plan.scratch(_e4m3_scratch_bytes(head_dim, n, n_q_heads, plan.max_len), q.device)
         rc = al.sb_attention_e4m3(
-            _ptr(q), _ptr(out), _code(q.dtype), n, plan.n_seqs, plan.max_new, plan.max_len, *_plan_pointers("attention_e4m3", plan, g),
-            g.page_size, _ptr(cache), _ptr(scales), cache.shape[0], n_q_heads, n_kv_heads, head_dim, window, scale, _ptr(scratch),
-            scratch.numel() if scratch is not None else 0, _stream())
+            rows, to, _code(dtype), n, plan.n_seqs, plan.max_new, plan.max_len, row0, pos0, off, ids, g.page_size, kept, kept_scales,
+            cache.shape[0], n_q_heads, n_kv_heads, head_dim, window, scale, scratch.data_ptr() if scratch is not None else None,
+            scratch.numel() if scratch is not None else 0, _stream_of(index))
         if rc != 0:
-            raise KernelError(f"attention_e4m3: {al.sb_last_error().decode()}")
+            raise KernelError(f"{what}: {al.sb_last_error().decode()}")
         LAUNCHES += 1 if scratch is None else 2
         return out
+    if values:
+        return _attention_of_values(q, out, plan, g, cache, scales, n_q_heads, n_kv_heads, head_dim, window, scale, index)
     _check(lib().sb_attention_e4m3_plain(
-        _ptr(q), _ptr(out), _code(q.dtype), n, _i32(plan.row_seq, "row_seq"), _i32(plan.row_pos, "row_pos"),
-        _i32(g.page_off, "page_off"), _i32(g.page_ids, "page_ids"), g.page_size, _ptr(cache), _ptr(scales), cache.shape[0], n_q_heads,
-        n_kv_heads, head_dim, window, ctypes.c_float(scale), _stream()), "attention_e4m3 (plain kernel)")
+        rows, to, _code(dtype), n, _i32(plan.row_seq, "row_seq"), _i32(plan.row_pos, "row_pos"), off, ids, g.page_size, kept, kept_scales,
+        cache.shape[0], n_q_heads, n_kv_heads, head_dim, window, scale, _stream_of(index)), "attention_e4m3 (plain kernel)")
     return out
 
 
@@ -843,18 +878,20 @@ class PageTables:
         self._pointers = [t.data_ptr() for t in (self.seq_row0, self.seq_pos0, self.row_seq, self.row_pos, self.row_slot,
                                                  self.page_off, self.page_ids, self.status)]
         self.seq_row0.zero_(), self.page_off.zero_(), self.status.zero_()
-        self.n_seqs, self.n_rows, self.max_pages, self.page_size, self.device = max_seqs, max_rows, max_pages, page_size, flat.device
+        self.n_seqs, self.n_rows, self.max_pages, self.page_size = max_seqs, max_rows, max_pages, page_size
+        self.device, self.index = flat.device, flat.get_device()
         self.max_new = self.max_len = 0
         self.groups = [TableGroup(self.page_off, self.page_ids, page_size)]
-        self._scratch = None
+        self._scratch = []
 
     def scratch(self, nbytes: int, device):
-        """Scratch memory shared by the step's kernels (made on first use, grown on demand); None when nothing is asked for."""
+        """Scratch memory shared by the step's kernels (made on first use, another one when more is asked for); None when nothing is.
+        The older ones stay: a graph that was captured with them may run again."""
         if nbytes <= 0:
             return None
-        if self._scratch is None or self._scratch.numel() < nbytes:
-            self._scratch = torch.empty(nbytes, dtype=torch.uint8, device=device)
-        return self._scratch
+        if not self._scratch or self._scratch[-1].numel() < nbytes:
+            self._scratch.append(torch.empty(nbytes, dtype=torch.uint8, device=device))
+        return self._scratch[-1]
 
     def check(self) -> None:
         """Raises KernelError where the last `page_tables` described no rows.  Waits for the device."""
@@ -876,18 +913,23 @@ def page_tables(slots: torch.Tensor, new: torch.Tensor, lengths: torch.Tensor, t
     place); rows behind the last sequence get 0, -1 and -1.  `max_new` and `max_len` bound every request's new tokens and its
     length after them.  All or nothing: where a request cannot be met `tables.status` says why and the tables describe no rows
     (`tables.check()` raises it).  Nothing is taken until `page_advance` records the step; called again before that, it gives the
-    same pages.  All arrays int32."""
-    n = tables.n_seqs
-    _on_current_device(lengths, "page_tables")
-    shape = table.shape
-    assert slots.numel() == new.numel() == n, f"page_tables: {slots.numel()} slots, {new.numel()} counts, tables for {n} requests"
-    assert len(shape) == 2 and lengths.numel() == shape[0] and n_free.numel() == 1 and tables.device == lengths.device
-    for t in (slots, new, lengths, table, free, n_free):
-        if t.dtype != torch.int32 or not t.is_cuda or not t.is_contiguous():
-            raise KernelError("page_tables: its arrays are contiguous int32 CUDA tensors")
+    same pages.  All arrays int32.
+
+    Kernels that read a plan ahead of their wait for the kernel before them (`attention` and `rope_store` of few rows) must not come
+    directly behind this one; those over an 8-bit cache and `rotation_table` may."""
+    what, n, shape = "page_tables", tables.n_seqs, table.shape
+    index = _device_of(lengths, what)
+    if not slots.numel() == new.numel() == n:
+        raise KernelError(f"{what}: {slots.numel()} slots, {new.numel()} counts, tables for {n} requests")
+    if len(shape) != 2 or lengths.numel() != shape[0] or n_free.numel() != 1 or tables.index != index:
+        raise KernelError(f"{what}: {lengths.numel()} lengths, a table of {tuple(shape)}, {n_free.numel()} counts of free pages, tables on {tables.device}")
+    if slots.dtype is not _I32T or new.dtype is not _I32T or lengths.dtype is not _I32T or table.dtype is not _I32T or free.dtype is not _I32T \
+            or n_free.dtype is not _I32T:
+        raise KernelError(f"{what}: all arrays are int32")
+    named, brought, held, pages, stack, top = _addresses(what, index, slots, new, lengths, table, free, n_free)
     _check(lib().sb_page_tables(
-        slots.data_ptr(), new.data_ptr(), n, lengths.data_ptr(), table.data_ptr(), *shape, free.data_ptr(), free.numel(), n_free.data_ptr(),
-        tables.page_size, tables.n_rows, tables.max_pages, max_new, max_len, *tables._pointers, _stream()), "page_tables")
+        named, brought, n, held, pages, *shape, stack, free.numel(), top, tables.page_size, tables.n_rows, tables.max_pages, max_new, max_len,
+        *tables._pointers, _stream_of(index)), what)
     tables.max_new, tables.max_len = max_new, max_len
     return tables
 
@@ -895,8 +937,9 @@ def page_tables(slots: torch.Tensor, new: torch.Tensor, lengths: torch.Tensor, t
 def page_advance(slots: torch.Tensor, new: torch.Tensor, lengths: torch.Tensor, n_free: torch.Tensor, tables: PageTables) -> None:
     """The step that `page_tables` of the same slots and counts described has run: its sequences grow, its pages are taken.
     Changes nothing where the tables have a status."""
-    assert slots.numel() == new.numel() == tables.n_seqs and n_free.numel() == 1
-    _on_current_device(lengths, "page_advance")
+    _device_of(lengths, "page_advance")
+    if not slots.numel() == new.numel() == tables.n_seqs or n_free.numel() != 1:
+        raise KernelError(f"page_advance: {slots.numel()} slots, {new.numel()} counts, tables for {tables.n_seqs} requests")
     _check(lib().sb_page_advance(_i32(slots, "slots"), _i32(new, "new"), tables.n_seqs, _i32(lengths, "lengths"), lengths.numel(),
                                  _i32(n_free, "n_free"), tables.page_size, _i32(tables.status, "status"), _stream()), "page_advance")
 
@@ -904,8 +947,9 @@ def page_advance(slots: torch.Tensor, new: torch.Tensor, lengths: torch.Tensor, 
 def page_release(slots: torch.Tensor, lengths: torch.Tensor, table: torch.Tensor, free: torch.Tensor, n_free: torch.Tensor,
                  page_size: int = 64) -> None:
     """The sequences in `slots` end: their pages go back on the stack and their lengths to 0."""
-    assert table.dim() == 2 and lengths.numel() == table.shape[0] and n_free.numel() == 1
-    _on_current_device(lengths, "page_release")
+    _device_of(lengths, "page_release")
+    if table.dim() != 2 or lengths.numel() != table.shape[0] or n_free.numel() != 1:
+        raise KernelError(f"page_release: {lengths.numel()} lengths, a table of {tuple(table.shape)}, {n_free.numel()} counts of free pages")
     _check(lib().sb_page_release(_i32(slots, "slots"), slots.numel(), _i32(lengths, "lengths"), _i32(table, "table"), table.shape[0],
                                  table.shape[1], _i32(free, "free"), free.numel(), _i32(n_free, "n_free"), page_size, _stream()),
            "page_release")

@@ -150,3 +150,19 @@ def test_device_pages_refuse_sizes_without_room():
     for sizes in ((0, 4, 4), (4, 0, 4), (4, 4, 0)):
         with pytest.raises(CacheError):
             DevicePages(*sizes, "cpu")
+
+
+def test_which_rows_attend_to_pages_as_they_are():
+    """A rule on sizes that needs no device: single tokens always, many bfloat16 rows by way of values, float32 rows as far as the
+    grid goes."""
+    class Plan:
+        def __init__(self, n_seqs, max_new, max_len):
+            self.n_seqs, self.max_new, self.max_len, self.n_rows = n_seqs, max_new, max_len, n_seqs * max_new
+
+    def direct(dtype, *plan):
+        return ops._reads_pages_directly(Plan(*plan), dtype, 28, 4, 128, 148)
+
+    bf16, f32 = torch.bfloat16, torch.float32
+    assert direct(bf16, 64, 1, 32768) and direct(bf16, 1, 2, 1 << 20) and direct(bf16, 1, 16, 16000) and direct(bf16, 8, 9, 4000)
+    assert not direct(bf16, 1, 2048, 2048) and not direct(bf16, 8, 64, 4000)
+    assert direct(f32, 1, 2048, 2048) and not direct(f32, 1, 65536, 65536) and not direct(f32, 1, 32768, 32768)

@@ -266,6 +266,59 @@ def test_attention_sees_a_nan_of_its_own_only():
         assert bool((got[0] == 1.0).all()) and bool(got[1, :2].isnan().all()) and bool((got[1, 2:] == 1.0).all())
 
 
+@pytest.mark.parametrize("hd,window", [(64, 0), (128, 0), (48, 0), (64, 3)])
+@pytest.mark.parametrize("kind", [0, 1])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_a_nan_reaches_the_rows_that_see_it(hd, window, kind, dtype):
+    """Several new rows of one sequence: a NaN in the key (or one value) at one of their positions, another one far back that only
+    an unbounded mask sees."""
+    hq, hkv, n, pos0, bad = 4, 1, 4, 70, 72
+    cache, scales = torch.ones(2, 2, hkv, PAGE, hd, device=DEV).to(torch.float8_e4m3fn), torch.ones(2, 2, hkv, device=DEV)
+    cache.view(torch.uint8)[1, kind, 0, bad - PAGE, 5] = 0xff
+    if window:
+        cache.view(torch.uint8)[1, :, 0, :67 - PAGE] = 0x7f
+    plan = Plan([n], [pos0], [[0, 1]])
+    out = torch.empty(n, hq * hd, dtype=dtype, device=DEV)
+    ops.attention_e4m3(torch.ones(n, hq, hd, dtype=dtype, device=DEV), out, plan, 0, cache, scales, hq, hkv, hd, window, 0.1, "few")
+    got = out.view(n, hq, hd).float().cpu()
+    for i in range(n):
+        sees = pos0 + i >= bad
+        if not sees:
+            assert bool((got[i] == 1.0).all()), i
+        elif kind == 0:
+            assert bool(got[i].isnan().all()), i
+        else:
+            assert bool(got[i, :, 5].isnan().all()) and int(got[i].isnan().sum()) == hq, i
+
+
+@pytest.mark.parametrize("page", [16, 48, 128])
+def test_pages_of_other_sizes(page):
+    """The store takes any, the plain attention and the one over values of float32 rows too."""
+    hq, hkv, hd, n, pos0 = 4, 2, 64, 150, 10
+    g = torch.Generator().manual_seed(page)
+    pages = [3, 0, 11, 5, 2, 1, 4, 7, 6, 8, 9][:-(-(n + pos0) // page)]
+    oracle = plain.PlainCache(12, hkv, hd, page)
+    cache = torch.zeros(12, 2, hkv, page, hd, dtype=torch.uint8, device=DEV).view(torch.float8_e4m3fn)
+    scales = torch.ones(12, 2, hkv, device=DEV)
+    for at, k in ((0, pos0), (pos0, n)):
+        plan = Plan([k], [at], [pages])
+        plan.groups[0].page_size = page
+        x = rows_of(k, hq, hkv, hd, g, 0.1 if at == 0 else 1.0)
+        q = torch.empty(k, hq, hd, device=DEV)
+        ops.rope_store_e4m3(x.view(k, -1).to(DEV), hq, hkv, hd, 0, None, plan, 0, cache, scales, q)
+        oracle.store(pages, at, torch.stack([x[:, hq:hq + hkv], x[:, hq + hkv:]], 1))
+    kv = oracle.keys_values(pages, n + pos0)
+    assert torch.equal(scales.cpu().double()[pages], oracle.scales[pages])
+    want, size, dots = plain.attend(q.double().cpu(), kv, pos0, 0, 0.125)
+    for kernel in ("plain", "values", "auto"):
+        out = torch.empty(n, hq * hd, device=DEV)
+        ops.attention_e4m3(q, out, plan, 0, cache, scales, hq, hkv, hd, 0, 0.125, kernel)
+        far = (out.cpu().double().view(n, hq, hd) - want).abs() / plain.tolerance(want, size, dots, 0.125, hd, n + pos0, torch.float32)
+        assert float(far.max()) <= 1.0, kernel
+    with pytest.raises(ops.KernelError):
+        ops.attention_e4m3(q, out, plan, 0, cache, scales, hq, hkv, hd, 0, 0.125, "few")
+
+
 def test_attention_without_pages_gives_zeros():
     cache, scales = device_cache(3, 1, 64)
     for new in ([1, 1], [40, 40]):
@@ -468,6 +521,8 @@ def test_refusals_in_python():
     qkv = torch.zeros(1, 4 * 64, device=DEV)
     good = (q, out, plan, 0, cache, scales, 2, 1, 64, 0, 0.1)
     ops.attention_e4m3(*good)
+    with pytest.raises(ops.KernelError):
+        ops.attention_e4m3(q, q, *good[2:])
     for i, bad in [(4, cache.float()), (4, cache[:, :, :, :32]), (5, scales.double()), (5, scales[:2]), (0, q.float()), (0, q[:, :1]), (6, 3), (8, 32)]:
         args = list(good)
         args[i] = bad

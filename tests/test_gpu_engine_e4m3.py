@@ -148,3 +148,23 @@ def test_device_pages():
     assert pages.lengths.tolist() == [3, 0, 65, 0] and int(pages.n_free) == 3
     pages.release(slots[:1])
     assert int(pages.n_free) == 5 and pages.free[:5].tolist() == [5, 4, 3, 0, 1] and pages.lengths.tolist() == [3, 0, 0, 0]
+
+
+def test_the_command_line(model_dirs, tmp_path, capsys):
+    from sonicboom_b200 import cli
+    prompts = prompts_for("B", [5, 70], seed=9)
+    tokens = tmp_path / "prompts.txt"
+    tokens.write_text("\n".join(" ".join(map(str, p)) for p in prompts))
+    assert cli.main(["generate", "-m", str(model_dirs["B"]), "--tokens", str(tokens), "-n", "6", "--ignore-eos", "--cache-dtype", "e4m3"]) == 0
+    got = [[int(t) for t in line.split()] for line in capsys.readouterr().out.strip().splitlines()]
+    model = llm.model_load(model_dirs["B"], dtype="bfloat16")
+    assert got == llm.generate_batch(model, prompts, max_tokens=6, ignore_eos=True, cache_dtype="e4m3")
+
+
+def test_a_graphs_scratch_outlives_a_larger_step():
+    """Tables that a graph was captured with serve a step that needs more scratch memory: the graph's own stays."""
+    from sonicboom_b200 import ops
+    t = ops.PageTables(1, 4, 4, "cuda:0")
+    a = t.scratch(100, "cuda:0")
+    b = t.scratch(1000, "cuda:0")
+    assert t.scratch(50, "cuda:0") is b and a.data_ptr() != b.data_ptr() and any(x is a for x in t._scratch)
