@@ -92,10 +92,12 @@ __global__ void __launch_bounds__(STORE_THREADS) store_kernel(const StoreArgs a)
 
 // The same for head sizes and rotated parts that are multiples of 8: a thread keeps eight values of up to P rows in registers (four
 // pairs four and four, or eight of the part beyond the rotation), so a value is read once, 16 bytes at a time, between the rotation,
-// the page's largest and the rounding.  Stretches of rows: 256 threads, several heads a block, which share the rows' angles in
-// registers (as many as leave every SM blocks); 2,048 rows of 28/4 heads of 128 14 us, 8.5 at the memory's pace, where a warp a row
-// with every value read twice took 47.  Up to STORE_FEW rows: a warp a head.
+// the page's largest and the rounding.  Stretches of rows: 256 threads, as many heads a block as leave every SM the two blocks that
+// its registers hold; the heads share the rows' angles in shared memory, and the next head's values are asked for before this
+// one's are written.  2,048 rows of 28/4 heads of 128 take 13.1 us, 8.5 at the memory's pace (47 with a warp a row and every value
+// read twice; 15 with values kept in shared memory for four blocks an SM).  Up to STORE_FEW rows: a warp a head.
 constexpr int MANY_THREADS = 256;
+constexpr int MANY_SMEM = 64 * 1024;              // the angles of a page of 64 tokens at rotated parts up to 256
 
 template <typename TQ>
 __device__ __forceinline__ void store_four(TQ* dst, const float* v);
@@ -115,6 +117,7 @@ __device__ __forceinline__ void load_four(float* v, const float* src) {
 
 template <int THREADS, int P, typename TQ>
 __global__ void __launch_bounds__(THREADS) store_many_kernel(const StoreArgs a, int heads_per_block) {
+  extern __shared__ __align__(16) float turns[];               // [row][rot]: the rows' angles
   __shared__ float warp_most[2][THREADS / 32];
   sb_pdl_launch();
   sb_pdl_wait();
@@ -125,92 +128,100 @@ __global__ void __launch_bounds__(THREADS) store_many_kernel(const StoreArgs a, 
   const int lo = max(pos0, start), hi = min(pos0 + n_new, start + a.page_size);       // positions
   if (lo >= hi) return;
   const int page = own_page(a.page_off, a.page_ids, seq, nth, a.n_pages);
-  const int units = a.hd / 8, per_pass = THREADS / units, u = tid % units, r = tid / units;
-  const int half = a.rot >> 1, pairs = a.rot / 8, n_heads = a.n_q_heads + 2 * a.n_kv_heads, width = n_heads * a.hd;
-  const bool turns = u < pairs;
-  const int e1 = turns ? 4 * u : a.rot + 8 * (u - pairs), e2 = turns ? e1 + half : e1 + 4;
+  const int units = a.hd / 8, per_pass = THREADS / units, u = tid % units, r = tid / units, first = row0 + lo - pos0;
+  const int half = a.rot >> 1, pairs = a.rot / 8, n_turned = a.n_q_heads + a.n_kv_heads, n_heads = n_turned + a.n_kv_heads;
+  const int e1 = u < pairs ? 4 * u : a.rot + 8 * (u - pairs), e2 = u < pairs ? e1 + half : e1 + 4;
   const int head0 = blockIdx.y * heads_per_block, head1 = min(head0 + heads_per_block, n_heads);
-  bool mine[P];
-  float cs[P][4], sn[P][4];
-#pragma unroll
-  for (int p = 0; p < P; ++p) {
-    const int at = r + p * per_pass;
-    mine[p] = r < per_pass && lo + at < hi;
-    if (mine[p] && turns && head0 < a.n_q_heads + a.n_kv_heads) {
-      const float* turn = a.angles + (size_t)(row0 + lo - pos0 + at) * a.rot + 4 * u;
-      load_four(cs[p], turn);
-      load_four(sn[p], turn + half);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) cs[p][i] = 1.0f, sn[p][i] = 0.0f;
-    }
-  }
-  for (int head = head0; head < head1; ++head) {
-    const bool is_q = head < a.n_q_heads, is_v = head >= a.n_q_heads + a.n_kv_heads;
-    if (!is_q && page < 0) return;               // no page of its own there: nothing is written
-    float x[P][8];
+  auto mine = [&](int p) { return r < per_pass && lo + r + p * per_pass < hi; };
+  auto load = [&](float (&x)[P][8], int head) {
 #pragma unroll
     for (int p = 0; p < P; ++p) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) x[p][i] = 0.0f;
-      if (mine[p]) {
-        const float* src = a.qkv + (size_t)(row0 + lo - pos0 + r + p * per_pass) * width + (size_t)head * a.hd;
+      if (mine(p)) {
+        const float* src = a.qkv + ((size_t)(first + r + p * per_pass) * n_heads + head) * a.hd;
         load_four(x[p], src + e1);
         load_four(x[p] + 4, src + e2);
       }
     }
-    if (turns && !is_v) {
+  };
+  float x[P][8];
+  load(x, head0);
+  const float* my_turns = a.angles + (size_t)first * a.rot;
+  if (THREADS > 32 && head0 < n_turned) {
+    for (int i = 4 * tid; i < (hi - lo) * a.rot; i += 4 * THREADS)
+      *reinterpret_cast<float4*>(turns + i) = *reinterpret_cast<const float4*>(my_turns + i);
+    my_turns = turns;
+    __syncthreads();
+  }
+  for (int head = head0; head < head1; ++head) {
+    const bool is_q = head < a.n_q_heads;
+    if (!is_q && page < 0) return;               // no page of its own there: nothing is written
+    float next[P][8];                            // the next head's values are on their way while this one's are written
+    if (THREADS > 32 && head + 1 < head1) load(next, head + 1);
+    if (u < pairs && head < n_turned) {
 #pragma unroll
       for (int p = 0; p < P; ++p)
+        if (mine(p)) {
+          float cs[4], sn[4];
+          load_four(cs, my_turns + (size_t)(r + p * per_pass) * a.rot + 4 * u);
+          load_four(sn, my_turns + (size_t)(r + p * per_pass) * a.rot + half + 4 * u);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float y = x[p][i], z = x[p][4 + i];
-          x[p][i] = sb_rot_lo(y, z, cs[p][i], sn[p][i]);
-          x[p][4 + i] = sb_rot_hi(y, z, cs[p][i], sn[p][i]);
+          for (int i = 0; i < 4; ++i) {
+            const float y = x[p][i], z = x[p][4 + i];
+            x[p][i] = sb_rot_lo(y, z, cs[i], sn[i]);
+            x[p][4 + i] = sb_rot_hi(y, z, cs[i], sn[i]);
+          }
         }
     }
     if (is_q) {
 #pragma unroll
       for (int p = 0; p < P; ++p)
-        if (mine[p]) {
-          TQ* dst = (TQ*)a.q_out + ((size_t)(row0 + lo - pos0 + r + p * per_pass) * a.n_q_heads + head) * a.hd;
+        if (mine(p)) {
+          TQ* dst = (TQ*)a.q_out + ((size_t)(first + r + p * per_pass) * a.n_q_heads + head) * a.hd;
           store_four<TQ>(dst + e1, x[p]);
           store_four<TQ>(dst + e2, x[p] + 4);
         }
-      continue;
-    }
-    const size_t block = (size_t)page * 2 * a.n_kv_heads + (head - a.n_q_heads);
-    uint8_t* dst = a.cache + block * a.page_size * a.hd;
-    const int before = lo > start ? exponent_of(a.scales[block]) : E4M3_LOWEST;        // of tokens of earlier steps
-    float most = 0.0f;
+    } else {
+      const size_t block = (size_t)page * 2 * a.n_kv_heads + (head - a.n_q_heads);
+      uint8_t* dst = a.cache + block * a.page_size * a.hd;
+      const int before = lo > start ? exponent_of(a.scales[block]) : E4M3_LOWEST;      // of tokens of earlier steps
+      float most = 0.0f;
 #pragma unroll
-    for (int p = 0; p < P; ++p)
+      for (int p = 0; p < P; ++p)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) most = fmaxf(most, e4m3_size(x[p][i]));
-    most = sb_warp_max(most);
-    float* shared = warp_most[head & 1];         // two of them: the next head's are written while these are read
-    if (lane == 0) shared[warp] = most;
-    __syncthreads();                             // and everybody has read the scale
+        for (int i = 0; i < 8; ++i) most = fmaxf(most, e4m3_size(x[p][i]));
+      most = sb_warp_max(most);
+      float* shared = warp_most[head & 1];       // two of them: the next head's are written while these are read
+      if (lane == 0) shared[warp] = most;
+      __syncthreads();                           // and everybody has read the scale
 #pragma unroll
-    for (int w = 0; w < THREADS / 32; ++w) most = fmaxf(most, shared[w]);
-    const int need = e4m3_exponent(most), e = max(need, before);
-    if (lo > start && e > before) {
-      const float shrink = exp2f((float)(before - e));
-      for (int i = 4 * tid; i < (lo - start) * a.hd; i += 4 * THREADS) {
-        const uint32_t v = *reinterpret_cast<const uint32_t*>(dst + i);
-        const float2 y = e4m3x2_to_float2(v & 0xffffu), z = e4m3x2_to_float2(v >> 16);
-        *reinterpret_cast<uint32_t*>(dst + i) = to_e4m3x2(y.x, y.y, shrink) | to_e4m3x2(z.x, z.y, shrink) << 16;
+      for (int w = 0; w < THREADS / 32; ++w) most = fmaxf(most, shared[w]);
+      const int e = max(e4m3_exponent(most), before);
+      if (lo > start && e > before) {
+        const float shrink = exp2f((float)(before - e));
+        for (int i = 4 * tid; i < (lo - start) * a.hd; i += 4 * THREADS) {
+          const uint32_t v = *reinterpret_cast<const uint32_t*>(dst + i);
+          const float2 y = e4m3x2_to_float2(v & 0xffffu), z = e4m3x2_to_float2(v >> 16);
+          *reinterpret_cast<uint32_t*>(dst + i) = to_e4m3x2(y.x, y.y, shrink) | to_e4m3x2(z.x, z.y, shrink) << 16;
+        }
       }
-    }
-    if (tid == 0) a.scales[block] = exp2_int(e);
-    const float inverse = exp2_int(-e);
+      if (tid == 0) a.scales[block] = exp2_int(e);
+      const float inverse = exp2_int(-e);
 #pragma unroll
-    for (int p = 0; p < P; ++p)
-      if (mine[p]) {
-        uint8_t* row = dst + (size_t)(lo - start + r + p * per_pass) * a.hd;
-        *reinterpret_cast<uint32_t*>(row + e1) = to_e4m3x2(x[p][0], x[p][1], inverse) | to_e4m3x2(x[p][2], x[p][3], inverse) << 16;
-        *reinterpret_cast<uint32_t*>(row + e2) = to_e4m3x2(x[p][4], x[p][5], inverse) | to_e4m3x2(x[p][6], x[p][7], inverse) << 16;
-      }
+      for (int p = 0; p < P; ++p)
+        if (mine(p)) {
+          uint8_t* row = dst + (size_t)(lo - start + r + p * per_pass) * a.hd;
+          *reinterpret_cast<uint32_t*>(row + e1) = to_e4m3x2(x[p][0], x[p][1], inverse) | to_e4m3x2(x[p][2], x[p][3], inverse) << 16;
+          *reinterpret_cast<uint32_t*>(row + e2) = to_e4m3x2(x[p][4], x[p][5], inverse) | to_e4m3x2(x[p][6], x[p][7], inverse) << 16;
+        }
+    }
+    if (THREADS > 32) {
+#pragma unroll
+      for (int p = 0; p < P; ++p)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[p][i] = next[p][i];
+    }
   }
 }
 
@@ -401,15 +412,25 @@ extern "C" int sb_rope_store_e4m3(const float* qkv, int n_rows, int n_seqs, int 
       (((uintptr_t)qkv | (uintptr_t)angles | (uintptr_t)q_out) & 15) == 0 && ((uintptr_t)cache & 3) == 0) {
     const bool few = max_new <= STORE_FEW && hd <= 256;
     const int per_pass = (few ? 32 : MANY_THREADS) / (hd / 8), rows = few ? max_new : page_size, passes = (rows + per_pass - 1) / per_pass;
-    const long blocks = (long)grid.x * n_heads * n_seqs, fill = blocks / (4L * (n_sms > 0 ? n_sms : 1));
+    const long blocks = (long)grid.x * n_heads * n_seqs, fill = blocks / (2L * (n_sms > 0 ? n_sms : 1));
     const int per_block = few ? 1 : (int)(fill < 1 ? 1 : fill > 8 ? 8 : fill);
-    if (passes <= 8) {
+    if (passes <= 8 && (few || (long)page_size * rot * 4 <= MANY_SMEM)) {
+      if (!few) {
+        cudaError_t e = cudaSuccess;
+        SB_DISPATCH_DTYPE(q_dtype, TQ, {
+          e = passes <= 2 ? sb_allow_shared<store_many_kernel<MANY_THREADS, 2, TQ>>(MANY_SMEM)
+                          : passes <= 4 ? sb_allow_shared<store_many_kernel<MANY_THREADS, 4, TQ>>(MANY_SMEM)
+                                        : sb_allow_shared<store_many_kernel<MANY_THREADS, 8, TQ>>(MANY_SMEM);
+        });
+        if (e != cudaSuccess) SB_FAIL(SB_ERR_CUDA, "%s: shared memory opt-in failed: %s", who, cudaGetErrorString(e));
+      }
       grid.y = (n_heads + per_block - 1) / per_block;
       SB_DISPATCH_DTYPE(q_dtype, TQ, {
         auto kernel = few ? (passes <= 1 ? store_many_kernel<32, 1, TQ> : passes <= 4 ? store_many_kernel<32, 4, TQ> : store_many_kernel<32, 8, TQ>)
                           : passes <= 2 ? store_many_kernel<MANY_THREADS, 2, TQ>
                                         : passes <= 4 ? store_many_kernel<MANY_THREADS, 4, TQ> : store_many_kernel<MANY_THREADS, 8, TQ>;
-        sb_launch<SB_K_ELEMENTWISE>(kernel, grid, dim3(few ? 32 : MANY_THREADS), 0, stream, a, per_block);
+        sb_launch<SB_K_ELEMENTWISE>(kernel, grid, dim3(few ? 32 : MANY_THREADS), few ? 0 : (size_t)page_size * rot * sizeof(float), stream, a,
+                                    per_block);
       });
       SB_CHECK_LAUNCH(who);
       return SB_OK;
