@@ -11,11 +11,23 @@ csrc/sonicboom_b200.h (and csrc/no_alloc.h); a test parses the headers and compa
 from __future__ import annotations
 
 import ctypes
+import struct
 
 CODES = {"i": ctypes.c_int, "f": ctypes.c_float, "z": ctypes.c_size_t, "u": ctypes.c_uint32,
          "p": ctypes.c_void_p, "s": ctypes.c_void_p, "c": ctypes.c_char_p, "v": None}
 
 _GEMM = "pipiiiiipippis"          # A, a_dtype, W, w_dtype, M, N, K, epilogue, bias, bias_dtype, residual, out, out_dtype, stream
+
+# Argument records of the header whose entry points are called once a layer or oftener: their fields in order, packed by
+# `pack[name](values...)` into bytes that an entry point takes as a pointer (a fraction of what as many ctypes arguments cost).
+RECORDS = {
+    "SbStoreE4m3": "ppppppppp" "iiiiiiiiiii",
+    "SbPageTables": "pppppppppppppp" "iiiiiiiii",
+    "SbAttentionE4m3": "ppppppppp" "z" "iiiiiiiiiii" "f",
+}
+_FORMAT = {"p": "P", "z": "N", "i": "i", "f": "f"}
+RECORD_STRUCTS = {name: struct.Struct("@" + "".join(_FORMAT[c] for c in codes)) for name, codes in RECORDS.items()}
+pack = {name: s.pack for name, s in RECORD_STRUCTS.items()}
 
 EVERY_LIBRARY = {
     "sb_last_error": ("c", ""),
@@ -100,10 +112,10 @@ CORE = {
     "sb_moe_join": ("i", "ppppfipippipiiiipis"),
     "sb_gemm_tc5_takes_angles": ("i", "iiiiiiiii"),
     "sb_rotation_table": ("i", "piipps"),
-    "sb_rope_store_e4m3": ("i", "piiiiiiipppppippipiis"),
+    "sb_rope_store_e4m3": ("i", "ps"),
     "sb_cache_e4m3_values": ("i", "ppiippiippiiiiipipps"),
     "sb_attention_e4m3_plain": ("i", "ppiippppippiiiiifs"),
-    "sb_page_tables": ("i", "ppippiipipiiiiipppppppps"),
+    "sb_page_tables": ("i", "ps"),
     "sb_page_advance": ("i", "ppipipips"),
     "sb_page_release": ("i", "pippiipipis"),
     "sb_sample_params_size": ("i", ""),
@@ -121,7 +133,7 @@ ATTENTION = {
     "sb_attention": ("i", "ppiiippppipiiiifpzpiiiipzpfipis"),
     "sb_attention_e4m3_status": ("i", ""),
     "sb_attention_e4m3_scratch_bytes": ("z", "iii"),
-    "sb_attention_e4m3": ("i", "ppiiiiippppippiiiiifpzs"),
+    "sb_attention_e4m3": ("i", "ps"),
     "sb_attention_decode_static": ("i", "ppiiippppipiiiifis"),
     "sb_attention_static_scratch_bytes": ("z", ""),
 }

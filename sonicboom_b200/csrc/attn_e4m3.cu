@@ -667,30 +667,32 @@ extern "C" size_t sb_attention_e4m3_scratch_bytes(int n_rows, int n_q_heads, int
   return n <= 1 || n_rows <= 0 || n_q_heads <= 0 ? 0 : (size_t)n_rows * n_q_heads * n * PART * sizeof(float);
 }
 
-extern "C" int sb_attention_e4m3(const void* q, void* out, int dtype, int n_rows, int n_seqs, int max_new, int max_len,
-                                 const int32_t* seq_row0, const int32_t* seq_pos0, const int32_t* page_off, const int32_t* page_ids,
-                                 int page_size, const void* cache, const float* scales, int n_pages, int n_q_heads, int n_kv_heads, int hd,
-                                 int window, float scale, void* scratch, size_t scratch_bytes, cudaStream_t stream) {
+extern "C" int sb_attention_e4m3(const SbAttentionE4m3* args, cudaStream_t stream) {
   const char* who = "sb_attention_e4m3";
-  if (hd != HD) SB_FAIL(SB_ERR_ARG, "%s: built for head size %d, called with %d", who, HD, hd);
-  if (page_size != PAGE) SB_FAIL(SB_ERR_UNSUPPORTED, "%s: cache pages of %d keys (needs %d)", who, page_size, PAGE);
-  if (!q || !out || !seq_row0 || !seq_pos0 || !page_off || !page_ids || !cache || !scales) SB_FAIL(SB_ERR_ARG, "%s: an array is missing", who);
-  if (n_rows <= 0 || n_seqs <= 0 || max_new <= 0 || max_len <= 0 || n_q_heads <= 0 || n_kv_heads <= 0 || n_pages <= 0)
-    SB_FAIL(SB_ERR_ARG, "%s: rows=%d seqs=%d max_new=%d max_len=%d heads=%d/%d pages=%d", who, n_rows, n_seqs, max_new, max_len, n_q_heads,
-            n_kv_heads, n_pages);
+  if (!args) SB_FAIL(SB_ERR_ARG, "%s: no arguments", who);
+  const SbAttentionE4m3 x = *args;
+  const int dtype = x.dtype, n_seqs = x.n_seqs, max_new = x.max_new, n_q_heads = x.n_q_heads, n_kv_heads = x.n_kv_heads;
+  if (x.hd != HD) SB_FAIL(SB_ERR_ARG, "%s: built for head size %d, called with %d", who, HD, x.hd);
+  if (x.page_size != PAGE) SB_FAIL(SB_ERR_UNSUPPORTED, "%s: cache pages of %d keys (needs %d)", who, x.page_size, PAGE);
+  if (!x.q || !x.out || !x.seq_row0 || !x.seq_pos0 || !x.page_off || !x.page_ids || !x.cache || !x.scales)
+    SB_FAIL(SB_ERR_ARG, "%s: an array is missing", who);
+  if (x.n_rows <= 0 || n_seqs <= 0 || max_new <= 0 || x.max_len <= 0 || n_q_heads <= 0 || n_kv_heads <= 0 || x.n_pages <= 0)
+    SB_FAIL(SB_ERR_ARG, "%s: rows=%d seqs=%d max_new=%d max_len=%d heads=%d/%d pages=%d", who, x.n_rows, n_seqs, max_new, x.max_len, n_q_heads,
+            n_kv_heads, x.n_pages);
   if (n_q_heads % n_kv_heads)
     SB_FAIL(SB_ERR_ARG, "%s: %d query heads are not a multiple of %d key/value heads", who, n_q_heads, n_kv_heads);
-  if (window < 0) SB_FAIL(SB_ERR_ARG, "%s: window %d (0: none)", who, window);
-  if ((((uintptr_t)q | (uintptr_t)cache | (uintptr_t)scratch) & 15) || ((uintptr_t)out & 15)) SB_FAIL(SB_ERR_ARG, "%s: unaligned operands", who);
+  if (x.window < 0) SB_FAIL(SB_ERR_ARG, "%s: window %d (0: none)", who, x.window);
+  if (((uintptr_t)x.q | (uintptr_t)x.cache | (uintptr_t)x.scratch | (uintptr_t)x.out) & 15) SB_FAIL(SB_ERR_ARG, "%s: unaligned operands", who);
   if (!sb_valid_dtype(dtype)) SB_FAIL(SB_ERR_ARG, "%s: dtype code %d", who, dtype);
   const long rows = (long)max_new * (n_q_heads / n_kv_heads), groups = row_groups(dtype, rows);
-  const long n_splits = most_splits(max_len), n_stretches = (n_splits + STRETCH - 1) / STRETCH;
+  const long n_splits = most_splits(x.max_len), n_stretches = (n_splits + STRETCH - 1) / STRETCH;
   if (groups * n_kv_heads > 65535 || n_seqs > 65535 || max_new > 65535 || n_stretches * PART * 4 > 48 * 1024)
-    SB_FAIL(SB_ERR_UNSUPPORTED, "%s: %d new rows of %d/%d heads, %d sequences, max_len %d", who, max_new, n_q_heads, n_kv_heads, n_seqs, max_len);
-  const size_t need = sb_attention_e4m3_scratch_bytes(n_rows, n_q_heads, max_len);
-  if (need > scratch_bytes || (need && !scratch)) SB_FAIL(SB_ERR_ARG, "%s: %zu bytes of scratch needed, %zu given", who, need, scratch_bytes);
-  const Args a = {q, out, seq_row0, seq_pos0, page_off, page_ids, (const uint8_t*)cache, scales, (float*)scratch,
-                  n_q_heads, n_kv_heads, n_pages, window, (int)n_splits, scale * LOG2E};
+    SB_FAIL(SB_ERR_UNSUPPORTED, "%s: %d new rows of %d/%d heads, %d sequences, max_len %d", who, max_new, n_q_heads, n_kv_heads, n_seqs, x.max_len);
+  const size_t need = sb_attention_e4m3_scratch_bytes(x.n_rows, n_q_heads, x.max_len);
+  if (need > x.scratch_bytes || (need && !x.scratch))
+    SB_FAIL(SB_ERR_ARG, "%s: %zu bytes of scratch needed, %zu given", who, need, x.scratch_bytes);
+  const Args a = {x.q, x.out, x.seq_row0, x.seq_pos0, x.page_off, x.page_ids, (const uint8_t*)x.cache, x.scales, (float*)x.scratch,
+                  n_q_heads, n_kv_heads, x.n_pages, x.window, (int)n_splits, x.scale * LOG2E};
   const dim3 grid((unsigned)n_splits, (unsigned)(groups * n_kv_heads), n_seqs);
   cudaError_t e = cudaSuccess;
 #if SB_HD <= 128

@@ -22,17 +22,8 @@ __device__ __forceinline__ int own_page(const int32_t* page_off, const int32_t* 
 constexpr int STORE_THREADS = 128;
 constexpr int STORE_FEW = 8;                      // new rows a sequence up to which a warp takes a head
 
-struct StoreArgs {
-  const float *qkv, *angles;                     // [rows][(q heads + 2 kv heads) hd]; [rows][rot]: cosines, then sines
-  const int32_t *seq_row0, *seq_pos0, *page_off, *page_ids;
-  uint8_t* cache;
-  float* scales;
-  void* q_out;
-  int n_q_heads, n_kv_heads, hd, rot, page_size, n_pages;
-};
-
 template <typename TQ>
-__global__ void __launch_bounds__(STORE_THREADS) store_kernel(const StoreArgs a) {
+__global__ void __launch_bounds__(STORE_THREADS) store_kernel(const SbStoreE4m3 a) {
   __shared__ float warp_most[STORE_THREADS / 32];
   sb_pdl_launch();
   sb_pdl_wait();
@@ -68,7 +59,7 @@ __global__ void __launch_bounds__(STORE_THREADS) store_kernel(const StoreArgs a)
 #pragma unroll
   for (int w = 0; w < STORE_THREADS / 32; ++w) most = fmaxf(most, warp_most[w]);
   const size_t block = (size_t)page * 2 * a.n_kv_heads + (head - a.n_q_heads);
-  uint8_t* dst = a.cache + block * a.page_size * a.hd;
+  uint8_t* dst = (uint8_t*)a.cache + block * a.page_size * a.hd;
   int e2 = e4m3_exponent(most);
   if (lo > start) {                              // the page holds tokens of earlier steps
     const int before = exponent_of(a.scales[block]);
@@ -116,7 +107,7 @@ __device__ __forceinline__ void load_four(float* v, const float* src) {
 }
 
 template <int THREADS, int P, typename TQ>
-__global__ void __launch_bounds__(THREADS) store_many_kernel(const StoreArgs a, int heads_per_block) {
+__global__ void __launch_bounds__(THREADS) store_many_kernel(const SbStoreE4m3 a, int heads_per_block) {
   extern __shared__ __align__(16) float turns[];               // [row][rot]: the rows' angles
   __shared__ float warp_most[2][THREADS / 32];
   sb_pdl_launch();
@@ -184,7 +175,7 @@ __global__ void __launch_bounds__(THREADS) store_many_kernel(const StoreArgs a, 
         }
     } else {
       const size_t block = (size_t)page * 2 * a.n_kv_heads + (head - a.n_q_heads);
-      uint8_t* dst = a.cache + block * a.page_size * a.hd;
+      uint8_t* dst = (uint8_t*)a.cache + block * a.page_size * a.hd;
       const int before = lo > start ? exponent_of(a.scales[block]) : E4M3_LOWEST;      // of tokens of earlier steps
       float most = 0.0f;
 #pragma unroll
@@ -389,27 +380,27 @@ attention_kernel(const TQ* q, TQ* out, const int32_t* row_seq, const int32_t* ro
 
 }  // namespace
 
-extern "C" int sb_rope_store_e4m3(const float* qkv, int n_rows, int n_seqs, int max_new, int n_q_heads, int n_kv_heads, int hd, int rot,
-                                  const float* angles, const int32_t* seq_row0, const int32_t* seq_pos0, const int32_t* page_off,
-                                  const int32_t* page_ids, int page_size, void* cache, float* scales, int n_pages, void* q_out, int q_dtype,
-                                  int n_sms, cudaStream_t stream) {
+extern "C" int sb_rope_store_e4m3(const SbStoreE4m3* args, cudaStream_t stream) {
   const char* who = "sb_rope_store_e4m3";
-  if (!qkv || !seq_row0 || !seq_pos0 || !page_off || !page_ids || !cache || !scales || !q_out) SB_FAIL(SB_ERR_ARG, "%s: an array is missing", who);
-  if (n_rows <= 0 || n_seqs <= 0 || max_new <= 0 || n_q_heads <= 0 || n_kv_heads <= 0 || page_size <= 0 || n_pages <= 0)
-    SB_FAIL(SB_ERR_ARG, "%s: rows=%d seqs=%d max_new=%d heads=%d/%d page=%d pages=%d", who, n_rows, n_seqs, max_new, n_q_heads, n_kv_heads,
-            page_size, n_pages);
+  if (!args) SB_FAIL(SB_ERR_ARG, "%s: no arguments", who);
+  const SbStoreE4m3 a = *args;
+  const int max_new = a.max_new, n_q_heads = a.n_q_heads, n_kv_heads = a.n_kv_heads, hd = a.hd, rot = a.rot, page_size = a.page_size;
+  if (!a.qkv || !a.seq_row0 || !a.seq_pos0 || !a.page_off || !a.page_ids || !a.cache || !a.scales || !a.q_out)
+    SB_FAIL(SB_ERR_ARG, "%s: an array is missing", who);
+  if (a.n_rows <= 0 || a.n_seqs <= 0 || max_new <= 0 || n_q_heads <= 0 || n_kv_heads <= 0 || page_size <= 0 || a.n_pages <= 0)
+    SB_FAIL(SB_ERR_ARG, "%s: rows=%d seqs=%d max_new=%d heads=%d/%d page=%d pages=%d", who, a.n_rows, a.n_seqs, max_new, n_q_heads, n_kv_heads,
+            page_size, a.n_pages);
   if (hd <= 0 || (hd & 1) || rot < 0 || rot > hd || (rot & 1))
     SB_FAIL(SB_ERR_ARG, "%s: rotary dims %d of head dim %d (both even, rotary dims at most the head dim)", who, rot, hd);
-  if (rot > 0 && !angles) SB_FAIL(SB_ERR_ARG, "%s: %d rotary dims without angles", who, rot);
-  if (!sb_valid_dtype(q_dtype)) SB_FAIL(SB_ERR_ARG, "%s: dtype code %d", who, q_dtype);
-  if (n_seqs > 65535 || n_q_heads + 2 * n_kv_heads > 65535)
-    SB_FAIL(SB_ERR_UNSUPPORTED, "%s: %d sequences, %d/%d heads", who, n_seqs, n_q_heads, n_kv_heads);
-  const StoreArgs a = {qkv, angles, seq_row0, seq_pos0, page_off, page_ids, (uint8_t*)cache, scales, q_out,
-                       n_q_heads, n_kv_heads, hd, rot, page_size, n_pages};
+  if (rot > 0 && !a.angles) SB_FAIL(SB_ERR_ARG, "%s: %d rotary dims without angles", who, rot);
+  if (!sb_valid_dtype(a.q_dtype)) SB_FAIL(SB_ERR_ARG, "%s: dtype code %d", who, a.q_dtype);
+  if (a.n_seqs > 65535 || (long)n_q_heads + 2L * n_kv_heads > 65535)
+    SB_FAIL(SB_ERR_UNSUPPORTED, "%s: %d sequences, %d/%d heads", who, a.n_seqs, n_q_heads, n_kv_heads);
+  const int n_seqs = a.n_seqs, n_sms = a.n_sms, q_dtype = a.q_dtype;
   const int n_heads = n_q_heads + 2 * n_kv_heads;
   dim3 grid((unsigned)(((long)max_new + 2 * page_size - 2) / page_size), n_heads, n_seqs);
   if (hd % 8 == 0 && rot % 8 == 0 && hd <= 8 * MANY_THREADS &&
-      (((uintptr_t)qkv | (uintptr_t)angles | (uintptr_t)q_out) & 15) == 0 && ((uintptr_t)cache & 3) == 0) {
+      (((uintptr_t)a.qkv | (uintptr_t)a.angles | (uintptr_t)a.q_out) & 15) == 0 && ((uintptr_t)a.cache & 3) == 0) {
     const bool few = max_new <= STORE_FEW && hd <= 256;
     const int per_pass = (few ? 32 : MANY_THREADS) / (hd / 8), rows = few ? max_new : page_size, passes = (rows + per_pass - 1) / per_pass;
     const long blocks = (long)grid.x * n_heads * n_seqs, fill = blocks / (2L * (n_sms > 0 ? n_sms : 1));

@@ -41,14 +41,7 @@ __device__ __forceinline__ int owner_of(const int* at, int n, int v) {
   return lo;
 }
 
-struct TableArgs {
-  const int32_t *slots, *fresh, *lengths, *free, *n_free;
-  int32_t* table;
-  int n_seqs, n_slots, width, n_pages, page_size, max_rows, max_pages, max_new, max_len;
-  int32_t *seq_row0, *seq_pos0, *row_seq, *row_pos, *row_slot, *page_off, *page_ids, *status;
-};
-
-__global__ void __launch_bounds__(TB) page_tables_kernel(const TableArgs a) {
+__global__ void __launch_bounds__(TB) page_tables_kernel(const SbPageTables a) {
   extern __shared__ __align__(16) int smem[];
   __shared__ Sums warp_sums[TB / 32];
   __shared__ int found;
@@ -251,29 +244,26 @@ int check_pool(const char* who, const void* slots, const void* lengths, const vo
 
 }  // namespace
 
-extern "C" int sb_page_tables(const int32_t* slots, const int32_t* fresh, int n_seqs, const int32_t* lengths, int32_t* table, int n_slots,
-                              int width, const int32_t* free, int n_pages, const int32_t* n_free, int page_size, int max_rows,
-                              int max_pages, int max_new, int max_len, int32_t* seq_row0, int32_t* seq_pos0, int32_t* row_seq,
-                              int32_t* row_pos, int32_t* row_slot, int32_t* page_off, int32_t* page_ids, int32_t* status,
-                              cudaStream_t stream) {
+extern "C" int sb_page_tables(const SbPageTables* args, cudaStream_t stream) {
   const char* who = "sb_page_tables";
-  if (int rc = check_pool(who, slots, lengths, n_free, n_seqs, n_slots, page_size)) return rc;
-  if (!fresh || !table || !free || !seq_row0 || !seq_pos0 || !row_seq || !row_pos || !row_slot || !page_off || !page_ids || !status)
+  if (!args) SB_FAIL(SB_ERR_ARG, "%s: no arguments", who);
+  const SbPageTables a = *args;
+  if (int rc = check_pool(who, a.slots, a.lengths, a.n_free, a.n_seqs, a.n_slots, a.page_size)) return rc;
+  if (!a.fresh || !a.table || !a.free || !a.seq_row0 || !a.seq_pos0 || !a.row_seq || !a.row_pos || !a.row_slot || !a.page_off || !a.page_ids ||
+      !a.status)
     SB_FAIL(SB_ERR_ARG, "%s: an array is missing", who);
-  if (width <= 0 || n_pages <= 0 || max_rows <= 0 || max_pages <= 0 || max_new <= 0 || max_len <= 0)
-    SB_FAIL(SB_ERR_ARG, "%s: %d pages a slot, %d pages, room for %d rows and %d pages, max_new %d, max_len %d", who, width, n_pages,
-            max_rows, max_pages, max_new, max_len);
-  if (width > MAX_COUNT || max_rows > MAX_COUNT || (long)n_pages * page_size > 2147483647L)
-    SB_FAIL(SB_ERR_UNSUPPORTED, "%s: %d pages a slot, %d rows (at most %d), %d pages of %d tokens (places are 32-bit numbers)", who, width,
-            max_rows, MAX_COUNT, n_pages, page_size);
-  const TableArgs a = {slots, fresh, lengths, free, n_free, table, n_seqs, n_slots, width, n_pages, page_size, max_rows, max_pages, max_new,
-                       max_len, seq_row0, seq_pos0, row_seq, row_pos, row_slot, page_off, page_ids, status};
+  if (a.width <= 0 || a.n_pages <= 0 || a.max_rows <= 0 || a.max_pages <= 0 || a.max_new <= 0 || a.max_len <= 0)
+    SB_FAIL(SB_ERR_ARG, "%s: %d pages a slot, %d pages, room for %d rows and %d pages, max_new %d, max_len %d", who, a.width, a.n_pages,
+            a.max_rows, a.max_pages, a.max_new, a.max_len);
+  if (a.width > MAX_COUNT || a.max_rows > MAX_COUNT || (long)a.n_pages * a.page_size > 2147483647L)
+    SB_FAIL(SB_ERR_UNSUPPORTED, "%s: %d pages a slot, %d rows (at most %d), %d pages of %d tokens (places are 32-bit numbers)", who, a.width,
+            a.max_rows, MAX_COUNT, a.n_pages, a.page_size);
   constexpr int MOST_SMEM = ((5 * MAX_SEQS + 2) + MAX_SLOTS / 32) * 4;
   static_assert(MOST_SMEM <= 226 * 1024, "the requests' numbers fit a block's shared memory");
   if (cudaError_t e = sb_allow_shared<page_tables_kernel>(MOST_SMEM))
     SB_FAIL(SB_ERR_CUDA, "%s: shared memory opt-in failed: %s", who, cudaGetErrorString(e));
-  const size_t smem = ((size_t)5 * n_seqs + 2 + (n_slots + 31) / 32) * 4;
-  const long chunks = (max_rows + CHUNK - 1) / CHUNK + ((long)max_pages + CHUNK - 1) / CHUNK;
+  const size_t smem = ((size_t)5 * a.n_seqs + 2 + (a.n_slots + 31) / 32) * 4;
+  const long chunks = (a.max_rows + CHUNK - 1) / CHUNK + ((long)a.max_pages + CHUNK - 1) / CHUNK;
   sb_launch<SB_K_OTHER>(page_tables_kernel, dim3((unsigned)(chunks < 256 ? chunks : 256)), dim3(TB), smem, stream, a);
   SB_CHECK_LAUNCH(who);
   return SB_OK;

@@ -495,10 +495,19 @@ int sb_random_normal(void* out, int out_dtype, size_t n, uint32_t key0, uint32_t
  * and k, v into the pages; rot 0: no rotation, angles may be null.  A page that holds tokens of earlier steps keeps them: its
  * numbers are brought to the new scale where that is larger.  A position without a page in its own sequence's list writes
  * nothing but its q; rows behind the last sequence are left as they are.  hd even. */
-int sb_rope_store_e4m3(const float* qkv, int n_rows, int n_seqs, int max_new, int n_q_heads, int n_kv_heads, int hd, int rot,
-                       const float* angles, const int32_t* seq_row0, const int32_t* seq_pos0, const int32_t* page_off,
-                       const int32_t* page_ids, int page_size, void* cache, float* scales, int n_pages, void* q_out, int q_dtype,
-                       int n_sms, sb_stream_t stream);
+typedef struct SbStoreE4m3 {
+  const float* qkv;
+  const float* angles;
+  const int32_t* seq_row0;
+  const int32_t* seq_pos0;
+  const int32_t* page_off;
+  const int32_t* page_ids;
+  void* cache;
+  float* scales;
+  void* q_out;
+  int n_rows, n_seqs, max_new, n_q_heads, n_kv_heads, hd, rot, page_size, n_pages, q_dtype, n_sms;
+} SbStoreE4m3;
+int sb_rope_store_e4m3(const SbStoreE4m3* args, sb_stream_t stream);
 /* The pages of a step's sequences as values (exactly), one after another as page_ids [n_list] lists them, [k|v][kv head][position]
  * [hd] each, with the page list numbers [n_list] that says so; 0 at positions that no row of the step sees.  Pages wholly before the window are left out.  Sequences whose positions
  * have no pages get zeros in out [rows][n_q_heads * hd], of the values' dtype: what attends to the values leaves them alone. */
@@ -524,10 +533,24 @@ enum SbTablesStatus {
   SB_TABLES_PAGE_LIST = 8,     /* more pages than max_pages */
   SB_TABLES_NO_PAGES = 16      /* more new pages than are free */
 };
-int sb_page_tables(const int32_t* slots, const int32_t* fresh, int n_seqs, const int32_t* lengths, int32_t* table, int n_slots, int width,
-                   const int32_t* free, int n_pages, const int32_t* n_free, int page_size, int max_rows, int max_pages, int max_new,
-                   int max_len, int32_t* seq_row0, int32_t* seq_pos0, int32_t* row_seq, int32_t* row_pos, int32_t* row_slot,
-                   int32_t* page_off, int32_t* page_ids, int32_t* status, sb_stream_t stream);
+typedef struct SbPageTables {
+  const int32_t* slots;
+  const int32_t* fresh;
+  const int32_t* lengths;
+  int32_t* table;
+  const int32_t* free;
+  const int32_t* n_free;
+  int32_t* seq_row0;
+  int32_t* seq_pos0;
+  int32_t* row_seq;
+  int32_t* row_pos;
+  int32_t* row_slot;
+  int32_t* page_off;
+  int32_t* page_ids;
+  int32_t* status;
+  int n_seqs, n_slots, width, n_pages, page_size, max_rows, max_pages, max_new, max_len;
+} SbPageTables;
+int sb_page_tables(const SbPageTables* args, sb_stream_t stream);
 /* The step that these tables described has run: lengths grow, n_free shrinks (neither where status is not 0). */
 int sb_page_advance(const int32_t* slots, const int32_t* fresh, int n_seqs, int32_t* lengths, int n_slots, int32_t* n_free, int page_size,
                     const int32_t* status, sb_stream_t stream);
@@ -560,10 +583,21 @@ int sb_attention(const void* q, void* out, int n_rows, int n_seqs, int max_new,
  * scratch of their own.  Rows behind the last sequence are left as they are. */
 int sb_attention_e4m3_status(void);       /* as sb_tc5_status */
 size_t sb_attention_e4m3_scratch_bytes(int n_rows, int n_q_heads, int max_len);
-int sb_attention_e4m3(const void* q, void* out, int dtype, int n_rows, int n_seqs, int max_new, int max_len, const int32_t* seq_row0,
-                      const int32_t* seq_pos0, const int32_t* page_off, const int32_t* page_ids, int page_size, const void* cache,
-                      const float* scales, int n_pages, int n_q_heads, int n_kv_heads, int hd, int window, float scale, void* scratch,
-                      size_t scratch_bytes, sb_stream_t stream);
+typedef struct SbAttentionE4m3 {
+  const void* q;
+  void* out;
+  const int32_t* seq_row0;
+  const int32_t* seq_pos0;
+  const int32_t* page_off;
+  const int32_t* page_ids;
+  const void* cache;
+  const float* scales;
+  void* scratch;
+  size_t scratch_bytes;
+  int dtype, n_rows, n_seqs, max_new, max_len, page_size, n_pages, n_q_heads, n_kv_heads, hd, window;
+  float scale;
+} SbAttentionE4m3;
+int sb_attention_e4m3(const SbAttentionE4m3* args, sb_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -675,6 +675,7 @@ E4M3 = torch.float8_e4m3fn
 
 
 _I32T, _F32T = torch.int32, torch.float32
+_pack_store, _pack_tables, _pack_attention = (_abi.pack[name] for name in ("SbStoreE4m3", "SbPageTables", "SbAttentionE4m3"))
 
 
 def _device_of(t, what) -> int:
@@ -741,15 +742,15 @@ def rope_store_e4m3(qkv: torch.Tensor, n_q_heads: int, n_kv_heads: int, head_dim
         raise KernelError(f"{what}: rows are {qkv.dtype} {tuple(qkv.shape)}, want float32 [{n}, {(n_q_heads + 2 * n_kv_heads) * head_dim}]")
     if q_out.numel() != n * n_q_heads * head_dim:
         raise KernelError(f"{what}: q_out is {tuple(q_out.shape)}, want [{n}, {n_q_heads}, {head_dim}]")
-    turn = None
+    turn = 0
     if angles is not None:
         if angles.dtype is not _F32T or angles.shape != (n, rotary_dim):
             raise KernelError(f"{what}: angles are {angles.dtype} {tuple(angles.shape)}, want float32 [{n}, {rotary_dim}]")
         (turn,) = _addresses(what, index, angles)
     rows, kept, kept_scales, q, row0, pos0, off, ids = _addresses(what, index, qkv, cache, scales, q_out, *_check_plan(what, plan, g))
-    _check(lib().sb_rope_store_e4m3(
-        rows, n, plan.n_seqs, plan.max_new, n_q_heads, n_kv_heads, head_dim, rotary_dim, turn, row0, pos0, off, ids, g.page_size, kept,
-        kept_scales, cache.shape[0], q, _code(q_out.dtype), _sm_count(index), _stream_of(index)), what)
+    _check(lib().sb_rope_store_e4m3(_pack_store(
+        rows, turn, row0, pos0, off, ids, kept, kept_scales, q, n, plan.n_seqs, plan.max_new, n_q_heads, n_kv_heads, head_dim, rotary_dim,
+        g.page_size, cache.shape[0], _code(q_out.dtype), _sm_count(index)), _stream_of(index)), what)
     return q_out
 
 
@@ -838,10 +839,10 @@ def attention_e4m3(q: torch.Tensor, out: torch.Tensor, plan, group_index: int, c
     if few:
         al = attention_lib(head_dim)
         scratch = plan.scratch(_e4m3_scratch_bytes(head_dim, n, n_q_heads, plan.max_len), q.device)
-        rc = al.sb_attention_e4m3(
-            rows, to, _code(dtype), n, plan.n_seqs, plan.max_new, plan.max_len, row0, pos0, off, ids, g.page_size, kept, kept_scales,
-            cache.shape[0], n_q_heads, n_kv_heads, head_dim, window, scale, scratch.data_ptr() if scratch is not None else None,
-            scratch.numel() if scratch is not None else 0, _stream_of(index))
+        rc = al.sb_attention_e4m3(_pack_attention(
+            rows, to, row0, pos0, off, ids, kept, kept_scales, scratch.data_ptr() if scratch is not None else 0,
+            scratch.numel() if scratch is not None else 0, _code(dtype), n, plan.n_seqs, plan.max_new, plan.max_len, g.page_size,
+            cache.shape[0], n_q_heads, n_kv_heads, head_dim, window, scale), _stream_of(index))
         if rc != 0:
             raise KernelError(f"{what}: {al.sb_last_error().decode()}")
         LAUNCHES += 1 if scratch is None else 2
@@ -927,9 +928,9 @@ def page_tables(slots: torch.Tensor, new: torch.Tensor, lengths: torch.Tensor, t
             or n_free.dtype is not _I32T:
         raise KernelError(f"{what}: all arrays are int32")
     named, brought, held, pages, stack, top = _addresses(what, index, slots, new, lengths, table, free, n_free)
-    _check(lib().sb_page_tables(
-        named, brought, n, held, pages, *shape, stack, free.numel(), top, tables.page_size, tables.n_rows, tables.max_pages, max_new, max_len,
-        *tables._pointers, _stream_of(index)), what)
+    _check(lib().sb_page_tables(_pack_tables(
+        named, brought, held, pages, stack, top, *tables._pointers, n, *shape, free.numel(), tables.page_size, tables.n_rows, tables.max_pages,
+        max_new, max_len), _stream_of(index)), what)
     tables.max_new, tables.max_len = max_new, max_len
     return tables
 

@@ -1,12 +1,14 @@
 """The 8-bit cache on a machine without a GPU: the plain form against torch's own e4m3, and what the entry points refuse before
 anything is launched (no address given here is one of a device: a call that is not refused would not come back with these codes)."""
 import math
+import re
+from pathlib import Path
 
 import pytest
 import torch
 
 import plain_cache_e4m3 as plain
-from sonicboom_b200 import ops
+from sonicboom_b200 import abi, ops
 
 ARG, UNSUPPORTED = 1, 2
 P = 4096                                                  # an address that nothing reads
@@ -40,10 +42,27 @@ def test_a_larger_scale_rounds_only_what_is_not_normal_any_more():
     assert float((before - after).abs().max()) <= 2.0 ** -10 * scale
 
 
+def record(name, *values):
+    return abi.pack[name](*(0 if v is None else v for v in values))
+
+
+def test_records_are_the_headers_structs():
+    text = re.sub(r"/\*.*?\*/", " ", (Path(abi.__file__).parent / "csrc" / "sonicboom_b200.h").read_text(), flags=re.S)
+    for name, codes in abi.RECORDS.items():
+        body = re.search(r"typedef struct %s \{(.*?)\} %s;" % (name, name), text, re.S).group(1)
+        found = ""
+        for decl in filter(None, (d.strip() for d in body.split(";"))):
+            code = "p" if "*" in decl else {"int": "i", "float": "f", "size_t": "z"}[decl.split()[0]]
+            found += code * (decl.count(",") + 1)
+        assert found == codes, name
+    for name in ("sb_rope_store_e4m3", "sb_page_tables"):
+        assert getattr(ops.lib(), name)(None, None) == ARG
+
+
 def store(l, qkv=P, rows=4, seqs=2, max_new=2, hq=4, hkv=2, hd=64, rot=64, angles=P, row0=P, pos0=P, off=P, ids=P, page=64, cache=P,
           scales=P, pages=8, q=P, dtype=1):
-    return l.sb_rope_store_e4m3(qkv, rows, seqs, max_new, hq, hkv, hd, rot, angles, row0, pos0, off, ids, page, cache, scales, pages, q, dtype,
-                                148, None)
+    return l.sb_rope_store_e4m3(record("SbStoreE4m3", qkv, angles, row0, pos0, off, ids, cache, scales, q, rows, seqs, max_new, hq, hkv, hd,
+                                       rot, page, pages, dtype, 148), None)
 
 
 @pytest.mark.parametrize("kw,code", [
@@ -85,8 +104,8 @@ def test_values_refusals(kw, code):
 
 def tables(l, slots=P, new=P, n=4, lengths=P, table=P, n_slots=8, width=4, free=P, pages=32, n_free=P, page=64, max_rows=16, max_pages=16,
            max_new=4, max_len=256, outs=(P,) * 8):
-    return l.sb_page_tables(slots, new, n, lengths, table, n_slots, width, free, pages, n_free, page, max_rows, max_pages, max_new, max_len,
-                            *outs, None)
+    return l.sb_page_tables(record("SbPageTables", slots, new, lengths, table, free, n_free, *outs, n, n_slots, width, pages, page, max_rows,
+                                   max_pages, max_new, max_len), None)
 
 
 @pytest.mark.parametrize("kw,code", [
@@ -166,3 +185,21 @@ def test_which_rows_attend_to_pages_as_they_are():
     assert direct(bf16, 64, 1, 32768) and direct(bf16, 1, 2, 1 << 20) and direct(bf16, 1, 16, 16000) and direct(bf16, 8, 9, 4000)
     assert not direct(bf16, 1, 2048, 2048) and not direct(bf16, 8, 64, 4000)
     assert direct(f32, 1, 2048, 2048) and not direct(f32, 1, 65536, 65536) and not direct(f32, 1, 32768, 32768)
+
+
+def attend_direct(l, q=P, out=2 * P, dtype=1, rows=4, seqs=2, max_new=2, max_len=100, row0=P, pos0=P, off=P, ids=P, page=64, cache=P, scales=P,
+                  pages=8, hq=4, hkv=2, hd=64, window=0, scratch=P, room=1 << 20):
+    return l.sb_attention_e4m3(record("SbAttentionE4m3", q, out, row0, pos0, off, ids, cache, scales, scratch, room, dtype, rows, seqs, max_new,
+                                      max_len, page, pages, hq, hkv, hd, window, 0.125), None)
+
+
+@pytest.mark.parametrize("kw,code", [
+    (dict(q=None), ARG), (dict(out=None), ARG), (dict(cache=None), ARG), (dict(scales=None), ARG), (dict(ids=None), ARG), (dict(rows=0), ARG),
+    (dict(seqs=0), ARG), (dict(max_new=0), ARG), (dict(max_len=0), ARG), (dict(pages=0), ARG), (dict(hq=5), ARG), (dict(window=-1), ARG),
+    (dict(dtype=2), ARG), (dict(hd=128), ARG), (dict(q=P + 8), ARG), (dict(scratch=P + 8), ARG), (dict(page=32), UNSUPPORTED),
+    (dict(seqs=65536), UNSUPPORTED), (dict(max_new=65536), UNSUPPORTED), (dict(max_len=2000, room=100), ARG),
+    (dict(max_len=2000, scratch=None), ARG), (dict(max_len=2 ** 31 - 1), UNSUPPORTED)])
+def test_attention_refusals(kw, code):
+    l = ops.attention_lib(64)
+    assert attend_direct(l, **kw) == code and b"sb_attention_e4m3" in l.sb_last_error()
+    assert l.sb_attention_e4m3(None, None) == ARG
