@@ -10,7 +10,7 @@
 // k-steps of S, 16 bytes of each of four values' rows for eight tiles of O.  A warp walks its pages alone: one bulk copy brings a
 // page's keys of the head, another its values, into the warp's own shared memory, and the next page's are asked for as soon as
 // the tile has been read.  (Copies of 16 bytes a lane, into registers or shared memory, kept the memory at 4.4 of the 6.1 TB/s
-// that bulk copies of the same pages reach: 64 sequences of 512 to 8,192 keys 78 to 80 us instead of 62.)
+// that bulk copies of the same pages reach: 64 sequences of 512 to 8,192 keys 78 to 80 us when bulk copies took 65.)
 // e4m3 to half is exact.  q is brought to halves with a power of two for each row: a bfloat16's 8 bits stay.  Weights are rounded
 // to halves (2^-11) after they were summed in float32, times 2^15 so that small ones stay normal numbers.  For float32 rows q and
 // the weights are two halves each, the second what the first left over (together within 2^-24 of a row's largest value, 2^-22
@@ -24,7 +24,7 @@
 // the pages' places: a block takes one split of one key/value head, warp w its pages w, w + 4, ..., merged in warp order; splits
 // are merged in ascending order by a second kernel.  (The block that is done last, by an arrival counter, took 3 us more than the
 // kernel's 2 at one sequence and as much more at 64; a cluster of the splits' blocks held shared memory for sequences with fewer
-// splits, 89 us instead of 62.)
+// splits, 89 us when this took 65.)
 #include "common.cuh"
 #include "e4m3.cuh"
 #include "tc5.cuh"
@@ -39,7 +39,19 @@ typedef __nv_bfloat16 bf16;
 constexpr int HD = SB_HD;
 constexpr int PAGE = 64;
 constexpr int WARPS = 4;
-constexpr int TILE = PAGE * HD;                  // bytes of a page's keys, or values, of one head: one copy
+constexpr int TILE = PAGE * HD;                  // bytes of a page's keys, or values, of one head
+// Step `sub` of a tile takes sixteen of its keys: slot m (row m of S^T, k = m of O^T) is key key_of(m) + sub STEP_KEYS for m < 8, slot
+// m + 8 the key HALF_KEYS behind slot m.  Where rows are 128 or 256 bytes, keys that lie as in memory begin at the same bank, and the
+// 16-byte reads of eight lanes meet twice (keys) and four times (values).  There a tile lies in four quarters of sixteen rows, each a
+// copy of its own, that start eight banks on from one another, and a step takes four keys of every quarter: the eight lanes read two
+// quarters two apart, or all four, and none meet (64 sequences of 512 to 8,192 keys, size 128: 65.2 to 61.2 us; size 256, 12,000 keys
+// each: 373 to 345).  At other sizes three more copies cost more than they save (80: 97 to 104 us; 64: 96.5 to 99.4), and a tile is
+// one copy with its keys in order.
+constexpr bool QUARTERS = HD % 128 == 0;
+constexpr int PIECES = QUARTERS ? 4 : 1, PIECE = TILE / PIECES, PIECE_SMEM = PIECE + (QUARTERS ? 32 : 0), TILE_SMEM = PIECES * PIECE_SMEM;
+constexpr int STEP_KEYS = QUARTERS ? 4 : 16, HALF_KEYS = QUARTERS ? 1 : 8;
+__device__ __forceinline__ int key_of(int m) { return QUARTERS ? 16 * (((m >> 1) + 2 * (m & 1)) & 3) + 2 * (m & 1) : m; }
+__device__ __forceinline__ int bytes_at(int key) { return key * HD + (QUARTERS ? (key >> 4) * 32 : 0); }
 constexpr int AHEAD = HD > 64 ? 1 : HD > 32 ? 2 : 4;         // pages whose tiles a warp has room for
 constexpr int PART = HD + 4;                     // floats of a split's partial row: o, m, l
 constexpr float LOG2E = 1.4426950408889634f;
@@ -64,8 +76,8 @@ struct Args {
 
 // Pages of a split of a sequence of this length.  Shorter splits give few sequences enough blocks, longer ones cost many sequences
 // less (a block's start and its partial rows).  Four, eight and sixteen pages at 28/4 heads of 128, us with the merge: one sequence of
-// 1,500 keys 7.2, 9.2, 12.6 and 64 of them 32.7, 29.6, 30.9; of 6,000 keys 7.3, 9.0, 12.6 and 95.6, 77.3, 73.7; one of 30,000
-// 16.3, 14.3, 13.9 and four of them 34.9, 30.1, 26.7.
+// 1,500 keys 7.5, 9.6, 12.8 and 64 of them 32.7, 28.9, 30.6; of 6,000 keys 7.7, 9.4, 13.1 and 92.4, 73.9, 71.6; one of 30,000
+// 17.6, 14.1, 14.7 and four of them 35.1, 28.2, 26.8.
 __host__ __device__ constexpr int split_pages(int len) {
   return len <= 2048 ? 4 : len <= 16384 ? 8 : len <= 131072 ? 16 : len <= 524288 ? 64 : 256;
 }
@@ -130,11 +142,12 @@ __device__ __forceinline__ void read_bytes(uint32_t* dst, const unsigned char* s
   }
 }
 
-// Keys 16 sub + g and 16 sub + g + 8 of a tile: thread t of a quad has bytes 16 t ... of every 64, 8 t ... of 32, 4 t ... of 16.
-__device__ __forceinline__ void read_keys(uint32_t (&w)[STEP_WORDS], const unsigned char* tile, int sub, int g, int t) {
+// The keys of slots g and g + 8 of step `sub`, whose slot g is at `mine` in step 0: thread t of a quad has bytes 16 t ...
+// of every 64, 8 t ... of 32, 4 t ... of 16.
+__device__ __forceinline__ void read_keys(uint32_t (&w)[STEP_WORDS], const unsigned char* mine, int sub, int t) {
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    const unsigned char* row = tile + (16 * sub + 8 * h + g) * HD;
+    const unsigned char* row = mine + (STEP_KEYS * sub + HALF_KEYS * h) * HD;
     uint32_t* dst = w + h * K_WORDS;
 #pragma unroll
     for (int c = 0; c < HD / 64; ++c) read_bytes<16>(dst + 4 * c, row + 64 * c + 16 * t);
@@ -142,11 +155,12 @@ __device__ __forceinline__ void read_keys(uint32_t (&w)[STEP_WORDS], const unsig
     if constexpr (N16) read_bytes<4>(dst + HD / 64 * 4 + 2 * N32, row + HD / 64 * 64 + 32 * N32 + 4 * t);
   }
 }
-// Values 16 sub + 2 t + {0, 1, 8, 9} of a tile: lane g has bytes 16 g ... of every 128, 8 g ... of 64, and so on.
-__device__ __forceinline__ void read_values(uint32_t (&w)[STEP_WORDS], const unsigned char* tile, int sub, int g, int t) {
+// The values of slots 2 t + {0, 1, 8, 9}, the first two at `even` and `odd` in step 0: lane g has bytes 16 g ... of every 128, 8 g ...
+// of 64, and so on.
+__device__ __forceinline__ void read_values(uint32_t (&w)[STEP_WORDS], const unsigned char* even, const unsigned char* odd, int sub, int g) {
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const unsigned char* row = tile + (16 * sub + 2 * t + (j & 1) + 8 * (j >> 1)) * HD;
+    const unsigned char* row = (j & 1 ? odd : even) + (STEP_KEYS * sub + HALF_KEYS * (j >> 1)) * HD;
     uint32_t* dst = w + j * V_WORDS;
 #pragma unroll
     for (int c = 0; c < N128; ++c) read_bytes<16>(dst + 4 * c, row + 128 * c + 16 * g);
@@ -261,13 +275,13 @@ __global__ void __launch_bounds__(WARPS * 32, HD <= 128 && NT == 1 && sizeof(T) 
   constexpr int ROWS = 8 * NT, PARTS = sizeof(T) / 2;
   const T* const q = (const T*)a.q;
   T* const out = (T*)a.out;
-  extern __shared__ __align__(128) unsigned char tiles[];           // [warp][AHEAD][k|v][TILE], then the warps' partial results
+  extern __shared__ __align__(128) unsigned char tiles[];           // [warp][AHEAD][k|v][TILE_SMEM], then the warps' partial results
   float(*part)[ROWS][PART] = reinterpret_cast<float(*)[ROWS][PART]>(tiles);
   __shared__ float stat_m[WARPS][ROWS], stat_l[WARPS][ROWS], stat_n[WARPS][ROWS];
   __shared__ __align__(8) uint64_t landed[WARPS][2 * AHEAD];
   __shared__ int failed;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-  const unsigned char* const my_tiles = tiles + warp * (2 * AHEAD * TILE);
+  const unsigned char* const my_tiles = tiles + warp * (2 * AHEAD * TILE_SMEM);
   const uint32_t ring = (uint32_t)__cvta_generic_to_shared(my_tiles);
   const uint32_t bars = (uint32_t)__cvta_generic_to_shared(landed[warp]);
   if (tid == 0) failed = 0;
@@ -301,16 +315,18 @@ __global__ void __launch_bounds__(WARPS * 32, HD <= 128 && NT == 1 && sizeof(T) 
   const int low = low_of(first_pos), high_low = low_of(last_pos);
   const int tile_lo = max(split * sq.sp, low / PAGE), tile_hi = min(split * sq.sp + sq.sp - 1, last_pos / PAGE);
   const int32_t* pages = a.page_ids + a.page_off[b];
-  // Page i of this warp's (i from 0) goes to place i mod AHEAD; lane 0 asks for its tiles, every lane waits for them.
+  // Page i of this warp's (i from 0) goes to places 2 (i mod AHEAD) and the next; lane 0 asks for its tiles, every lane waits for them.
   const int n_tiles = (tile_hi - tile_lo - warp + WARPS) / WARPS;   // none or less: no page is this warp's
   const size_t kind = (size_t)a.n_kv_heads * TILE;
   auto page_at = [&](int i) { return min(max(pages[tile_lo + warp + i * WARPS], 0), a.n_pages - 1); };
   auto ask = [&](int i, int page, int v) {
-    const uint32_t place = 2 * (i % AHEAD) + v;
+    const uint32_t at = 2 * (i % AHEAD) + v;
     const uint8_t* src = a.cache + ((size_t)page * 2 * a.n_kv_heads + kvh) * TILE + v * kind;
-    mbar_expect_tx(bars + 8 * place, TILE);
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n" ::"r"(ring + place * TILE),
-                 "l"(src), "n"(TILE), "r"(bars + 8 * place) : "memory");
+    mbar_expect_tx(bars + 8 * at, TILE);
+#pragma unroll
+    for (int c = 0; c < PIECES; ++c)
+      asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n" ::"r"(
+                       ring + at * TILE_SMEM + c * PIECE_SMEM), "l"(src + c * PIECE), "n"(PIECE), "r"(bars + 8 * at) : "memory");
   };
   const size_t scale_stride = 2 * (size_t)a.n_kv_heads;
   int page = n_tiles > 0 ? page_at(0) : 0;
@@ -323,6 +339,7 @@ __global__ void __launch_bounds__(WARPS * 32, HD <= 128 && NT == 1 && sizeof(T) 
         ask(i, p, 1);
       }
   }
+  const int own_key = key_of(g), even_key = key_of(2 * t), odd_key = key_of(2 * t + 1);
   float k_scale = a.scales[page * scale_stride + kvh], v_scale = a.scales[page * scale_stride + a.n_kv_heads + kvh];
 
   uint32_t qf[NT][HD / 16][2][PARTS];
@@ -357,11 +374,11 @@ __global__ void __launch_bounds__(WARPS * 32, HD <= 128 && NT == 1 && sizeof(T) 
     }
   int i = 0, gave_up = 0;                        // 1: at a page's keys, 2: at its values
   for (; i < n_tiles; ++i) {
-    const uint32_t place = 2 * (i % AHEAD), parity = i / AHEAD & 1;
+    const uint32_t at = 2 * (i % AHEAD), parity = i / AHEAD & 1;
     const int next = i + 1 < n_tiles ? page_at(i + 1) : page, ahead = i + AHEAD < n_tiles ? page_at(i + AHEAD) : 0;
     const float next_k = a.scales[next * scale_stride + kvh], next_v = a.scales[next * scale_stride + a.n_kv_heads + kvh];
     const int e = exponent_of(v_scale);
-    if (!__all_sync(0xffffffffu, mbar_wait(bars + 8 * place, parity, 31))) {
+    if (!__all_sync(0xffffffffu, mbar_wait(bars + 8 * at, parity, 31))) {
       gave_up = 1;
       break;
     }
@@ -370,7 +387,7 @@ __global__ void __launch_bounds__(WARPS * 32, HD <= 128 && NT == 1 && sizeof(T) 
 #pragma unroll
       for (int sub = 0; sub < 4; ++sub) {
         uint32_t w[STEP_WORDS];
-        read_keys(w, my_tiles + place * TILE, sub, g, t);
+        read_keys(w, my_tiles + at * TILE_SMEM + bytes_at(own_key), sub, t);
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -407,7 +424,7 @@ __global__ void __launch_bounds__(WARPS * 32, HD <= 128 && NT == 1 && sizeof(T) 
           if (!whole)
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-              const int key = key0 + 8 * j + g;
+              const int key = key0 + own_key + STEP_KEYS * (j >> 1) + HALF_KEYS * (j & 1);
               if (key > row_pos[n][r] || key < row_low[n][r]) s[n][j >> 1][2 * (j & 1) + r] = -INFINITY;
             }
 #pragma unroll
@@ -462,21 +479,21 @@ __global__ void __launch_bounds__(WARPS * 32, HD <= 128 && NT == 1 && sizeof(T) 
           }
         }
       }
-      if (!__all_sync(0xffffffffu, mbar_wait(bars + 8 * (place + 1), parity, 32))) {
+      if (!__all_sync(0xffffffffu, mbar_wait(bars + 8 * (at + 1), parity, 32))) {
         gave_up = 2;
         break;
       }
 #pragma unroll
       for (int sub = 0; sub < 4; ++sub) {
         uint32_t w[STEP_WORDS];
-        read_values(w, my_tiles + (place + 1) * TILE, sub, g, t);
+        read_values(w, my_tiles + (at + 1) * TILE_SMEM + bytes_at(even_key), my_tiles + (at + 1) * TILE_SMEM + bytes_at(odd_key), sub, g);
         if (!whole) {
           // Values that no row sees may hold anything, and 0 * NaN is NaN: they become 0.  A NaN that some rows see and others do
           // not goes to those that see it: it becomes 0 too, and a product of "is NaN" with "is seen" finds its rows.
           uint32_t nans = 0;
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            const int key = key0 + 16 * sub + 2 * t + (j & 1) + 8 * (j >> 1);
+            const int key = key0 + (j & 1 ? odd_key : even_key) + STEP_KEYS * sub + HALF_KEYS * (j >> 1);
             const bool seen = key <= last_pos && key >= low;
 #pragma unroll
             for (int i = 0; i < V_WORDS; ++i) {
@@ -499,8 +516,8 @@ __global__ void __launch_bounds__(WARPS * 32, HD <= 128 && NT == 1 && sizeof(T) 
               const int row = row_base + 8 * n + g, pos = row < R ? sq.pos0 + row / G : -1, lo = low_of(pos);
 #pragma unroll
               for (int h = 0; h < 2; ++h) {
-                const int key = key0 + 16 * sub + 2 * t + 8 * h;
-                sees[n][h][0] = (key <= pos && key >= lo ? 0x3c00u : 0u) | (key + 1 <= pos && key + 1 >= lo ? 0x3c000000u : 0u);
+                const int first = key0 + STEP_KEYS * sub + HALF_KEYS * h, even = first + even_key, odd = first + odd_key;
+                sees[n][h][0] = (even <= pos && even >= lo ? 0x3c00u : 0u) | (odd <= pos && odd >= lo ? 0x3c000000u : 0u);
               }
             }
             values_step<NT, 1>(count, is_nan, sees);
@@ -648,7 +665,7 @@ __global__ void __launch_bounds__(HD / 4 * MOST_GROUPS) attn_e4m3_merge_kernel(c
 
 template <int NT, typename T>
 cudaError_t launch(const Args& a, dim3 grid, cudaStream_t stream) {
-  constexpr int TILES = WARPS * 2 * AHEAD * TILE, PARTIALS = WARPS * 8 * NT * PART * 4, SMEM = TILES > PARTIALS ? TILES : PARTIALS;
+  constexpr int TILES = WARPS * 2 * AHEAD * TILE_SMEM, PARTIALS = WARPS * 8 * NT * PART * 4, SMEM = TILES > PARTIALS ? TILES : PARTIALS;
   if (cudaError_t e = sb_allow_shared<attn_e4m3_kernel<NT, T>>(SMEM)) return e;
   return sb_launch<SB_K_ATTENTION>(attn_e4m3_kernel<NT, T>, grid, dim3(WARPS * 32), SMEM, stream, a);
 }
