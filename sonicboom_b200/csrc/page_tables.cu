@@ -30,6 +30,9 @@ __device__ __forceinline__ Sums up(Sums v, int o) {
   return {__shfl_up_sync(0xffffffffu, v.rows, o), __shfl_up_sync(0xffffffffu, v.total, o), __shfl_up_sync(0xffffffffu, v.taken, o)};
 }
 
+// Pages of so many tokens (0 or more, up to the largest int).
+__device__ __forceinline__ int pages_of(int tokens, int page_size) { return tokens > 0 ? (tokens - 1) / page_size + 1 : 0; }
+
 // The last i with at[i] <= v, of n + 1 ascending numbers with at[0] <= v < at[n].
 __device__ __forceinline__ int owner_of(const int* at, int n, int v) {
   int lo = 0, hi = n;
@@ -75,7 +78,7 @@ __global__ void __launch_bounds__(TB) page_tables_kernel(const SbPageTables a) {
         if (held < 0 || fresh > a.max_new || len > a.max_len || len > (long long)a.width * a.page_size) bad = SB_TABLES_TOO_LONG;
       }
       if (bad) fresh = held = 0;
-      const int have = (held + a.page_size - 1) / a.page_size, total = (held + fresh + a.page_size - 1) / a.page_size;
+      const int have = pages_of(held, a.page_size), total = pages_of(held + fresh, a.page_size);
       v = {min(fresh, a.max_rows + 1), total, total - have};
       length[i] = held;
       slot_of[i] = bad ? 0 : slot;
@@ -123,7 +126,7 @@ __global__ void __launch_bounds__(TB) page_tables_kernel(const SbPageTables a) {
   const int n_rows = row0[a.n_seqs], n_list = off[a.n_seqs];
   // page i of a request: held, or the next one of the stack
   auto page_of = [&](int s, int i) {
-    const int have = (length[s] + a.page_size - 1) / a.page_size;
+    const int have = pages_of(length[s], a.page_size);
     return i < have ? a.table[(size_t)slot_of[s] * a.width + i] : a.free[n_free - 1 - (taken[s] + i - have)];
   };
   const int row_chunks = (a.max_rows + CHUNK - 1) / CHUNK, chunks = row_chunks + (n_list + CHUNK - 1) / CHUNK;
@@ -146,7 +149,7 @@ __global__ void __launch_bounds__(TB) page_tables_kernel(const SbPageTables a) {
       for (int k = (c - row_chunks) * CHUNK + tid; k < end; k += TB) {
         const int s = owner_of(off, a.n_seqs, k), i = k - off[s], page = page_of(s, i);
         a.page_ids[k] = page;
-        if (i >= (length[s] + a.page_size - 1) / a.page_size) a.table[(size_t)slot_of[s] * a.width + i] = page;
+        if (i >= pages_of(length[s], a.page_size)) a.table[(size_t)slot_of[s] * a.width + i] = page;
       }
     }
   }
@@ -165,7 +168,7 @@ __global__ void __launch_bounds__(TB) page_advance_kernel(const int32_t* slots, 
     const int slot = slots[i];
     if (slot < 0 || slot >= n_slots) continue;
     const int held = lengths[slot], len = held + fresh[i];
-    mine += (len + page_size - 1) / page_size - (held + page_size - 1) / page_size;
+    mine += pages_of(len, page_size) - pages_of(held, page_size);
     lengths[slot] = len;
   }
   if (mine) atomicAdd(&taken, mine);             // whole numbers: the order does not matter
@@ -189,7 +192,7 @@ __global__ void __launch_bounds__(TB) page_release_kernel(const int32_t* slots, 
     if (slot >= 0 && slot < n_slots && atomicOr(&released[slot >> 5], 1u << (slot & 31)) >> (slot & 31) & 1) twice = 1;
   }
   __syncthreads();
-  int top = n_free[0];
+  int top = min(max(n_free[0], 0), n_pages);     // at most n_pages at all times, whatever lengths say
   for (int first = 0; first < n_seqs; first += TB) {
     const int i = first + tid;
     int slot = -1, count = 0;
@@ -199,7 +202,7 @@ __global__ void __launch_bounds__(TB) page_release_kernel(const int32_t* slots, 
       if (twice)                                 // some slot is: who is named before looks for itself
         for (int j = 0; j < i; ++j)
           if (slots[j] == slot) slot = -1;
-      if (slot >= 0) count = min((max(lengths[slot], 0) + page_size - 1) / page_size, width);
+      if (slot >= 0) count = min(pages_of(lengths[slot], page_size), width);
     }
     int mine = count;
 #pragma unroll
@@ -216,21 +219,21 @@ __global__ void __launch_bounds__(TB) page_release_kernel(const int32_t* slots, 
       tile += warp_sums[w];
     }
     // a warp takes its sequences one after another, so that a long one's pages move together
-    const int at = top + before + mine - count;
+    const int at = (int)min((long long)top + before + mine - count, (long long)n_pages);
     for (int l = 0; l < 32; ++l) {
       const int s = __shfl_sync(0xffffffffu, slot, l), n = __shfl_sync(0xffffffffu, count, l), to = __shfl_sync(0xffffffffu, at, l);
       if (s < 0) continue;
       for (int k = lane; k < n; k += 32) {
         const size_t from = (size_t)s * width + k;
-        if (to + k < n_pages) free[to + k] = table[from];
+        if (k < n_pages - to) free[to + k] = table[from];
         table[from] = -1;
       }
       if (lane == 0) lengths[s] = 0;
     }
-    top += tile;
+    top = (int)min((long long)top + tile, (long long)n_pages);
     __syncthreads();
   }
-  if (tid == 0) n_free[0] = min(top, n_pages);
+  if (tid == 0) n_free[0] = top;
 }
 
 int check_pool(const char* who, const void* slots, const void* lengths, const void* n_free, int n_seqs, int n_slots, int page_size) {
@@ -285,6 +288,7 @@ extern "C" int sb_page_release(const int32_t* slots, int n_seqs, int32_t* length
   const char* who = "sb_page_release";
   if (int rc = check_pool(who, slots, lengths, n_free, n_seqs, n_slots, page_size)) return rc;
   if (!table || !free || width <= 0 || n_pages <= 0) SB_FAIL(SB_ERR_ARG, "%s: %d pages a slot, %d pages, or an array is missing", who, width, n_pages);
+  if (width > MAX_COUNT) SB_FAIL(SB_ERR_UNSUPPORTED, "%s: %d pages a slot (at most %d)", who, width, MAX_COUNT);
   sb_launch<SB_K_OTHER>(page_release_kernel, dim3(1), dim3(TB), (size_t)((n_slots + 31) / 32) * 4, stream, slots, n_seqs, n_slots, lengths,
                         table, width, free, n_pages, n_free, page_size);
   SB_CHECK_LAUNCH(who);
