@@ -64,7 +64,7 @@ __global__ void __launch_bounds__(STORE_THREADS) store_kernel(const SbStoreE4m3 
   if (lo > start) {                              // the page holds tokens of earlier steps
     const int before = exponent_of(a.scales[block]);
     if (e2 > before) {
-      const float shrink = exp2f((float)(before - e2));
+      const float shrink = exp2_int(max(before - e2, -126));     // 2^-126 and less: nothing of a number is left
       for (int i = 2 * tid; i < (lo - start) * a.hd; i += 2 * STORE_THREADS) {
         const float2 v = e4m3x2_to_float2(*reinterpret_cast<const uint16_t*>(dst + i));
         *reinterpret_cast<uint16_t*>(dst + i) = (uint16_t)to_e4m3x2(v.x, v.y, shrink);
@@ -190,7 +190,7 @@ __global__ void __launch_bounds__(THREADS) store_many_kernel(const SbStoreE4m3 a
       for (int w = 0; w < THREADS / 32; ++w) most = fmaxf(most, shared[w]);
       const int e = max(e4m3_exponent(most), before);
       if (lo > start && e > before) {
-        const float shrink = exp2f((float)(before - e));
+        const float shrink = exp2_int(max(before - e, -126));      // 2^-126 and less: nothing of a number is left
         for (int i = 4 * tid; i < (lo - start) * a.hd; i += 4 * THREADS) {
           const uint32_t v = *reinterpret_cast<const uint32_t*>(dst + i);
           const float2 y = e4m3x2_to_float2(v & 0xffffu), z = e4m3x2_to_float2(v >> 16);
@@ -263,7 +263,10 @@ values_kernel(const int32_t* seq_row0, const int32_t* seq_pos0, const int32_t* p
   }
   const int start = i * page_size, low = window > 0 ? max(0, pos0 - window + 1) : 0;
   if (start >= len || first + i >= n_list) return;
-  if (head == 0 && tid == 0) numbers[first + i] = first + i;
+  if (head == 0 && tid == 0) {
+    numbers[first + i] = first + i;
+    __threadfence();                             // a successor may read it ahead of its wait, once this grid's blocks are done
+  }
   if (start + page_size <= low) return;
   const int page = min(max(page_ids[first + i], 0), n_pages - 1);
   const size_t block = (size_t)page * gridDim.y + head;

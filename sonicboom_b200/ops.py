@@ -703,6 +703,10 @@ def _addresses(what, index, *tensors):
     return found
 
 
+def _overlap(a, a_address, b, b_address) -> bool:
+    return a_address < b_address + b.numel() * b.element_size() and b_address < a_address + a.numel() * a.element_size()
+
+
 def _check_plan(what, plan, g):
     """The arrays of a plan that kernels over an 8-bit cache read: row and position offsets, a group's page list."""
     row0, pos0, off, ids = arrays = plan.seq_row0, plan.seq_pos0, g.page_off, g.page_ids
@@ -748,6 +752,8 @@ def rope_store_e4m3(qkv: torch.Tensor, n_q_heads: int, n_kv_heads: int, head_dim
             raise KernelError(f"{what}: angles are {angles.dtype} {tuple(angles.shape)}, want float32 [{n}, {rotary_dim}]")
         (turn,) = _addresses(what, index, angles)
     rows, kept, kept_scales, q, row0, pos0, off, ids = _addresses(what, index, qkv, cache, scales, q_out, *_check_plan(what, plan, g))
+    if _overlap(qkv, rows, q_out, q):
+        raise KernelError(f"{what}: the rows and q_out share memory")
     _check(lib().sb_rope_store_e4m3(_pack_store(
         rows, turn, row0, pos0, off, ids, kept, kept_scales, q, n, plan.n_seqs, plan.max_new, n_q_heads, n_kv_heads, head_dim, rotary_dim,
         g.page_size, cache.shape[0], _code(q_out.dtype), _sm_count(index)), _stream_of(index)), what)
@@ -827,7 +833,7 @@ def attention_e4m3(q: torch.Tensor, out: torch.Tensor, plan, group_index: int, c
         raise KernelError(f"{what}: {n_q_heads} query heads are not a multiple of {n_kv_heads} key/value heads")
     few = values = False
     rows, to, kept, kept_scales, row0, pos0, off, ids = _addresses(what, index, q, out, cache, scales, *_check_plan(what, plan, g))
-    if to == rows:
+    if _overlap(q, rows, out, to):
         raise KernelError(f"{what}: q and out share memory: a row's query is read by several blocks until the last one is done")
     if kernel != "plain" and (rows | to | kept) % 16 == 0:
         few = head_dim % 16 == 0 and 16 <= head_dim <= 256 and g.page_size == 64
@@ -938,9 +944,10 @@ def page_tables(slots: torch.Tensor, new: torch.Tensor, lengths: torch.Tensor, t
 def page_advance(slots: torch.Tensor, new: torch.Tensor, lengths: torch.Tensor, n_free: torch.Tensor, tables: PageTables) -> None:
     """The step that `page_tables` of the same slots and counts described has run: its sequences grow, its pages are taken.
     Changes nothing where the tables have a status."""
-    _device_of(lengths, "page_advance")
+    index = _device_of(lengths, "page_advance")
     if not slots.numel() == new.numel() == tables.n_seqs or n_free.numel() != 1:
         raise KernelError(f"page_advance: {slots.numel()} slots, {new.numel()} counts, tables for {tables.n_seqs} requests")
+    _addresses("page_advance", index, slots, new, n_free, tables.status)
     _check(lib().sb_page_advance(_i32(slots, "slots"), _i32(new, "new"), tables.n_seqs, _i32(lengths, "lengths"), lengths.numel(),
                                  _i32(n_free, "n_free"), tables.page_size, _i32(tables.status, "status"), _stream()), "page_advance")
 
@@ -948,9 +955,10 @@ def page_advance(slots: torch.Tensor, new: torch.Tensor, lengths: torch.Tensor, 
 def page_release(slots: torch.Tensor, lengths: torch.Tensor, table: torch.Tensor, free: torch.Tensor, n_free: torch.Tensor,
                  page_size: int = 64) -> None:
     """The sequences in `slots` end: their pages go back on the stack and their lengths to 0."""
-    _device_of(lengths, "page_release")
+    index = _device_of(lengths, "page_release")
     if table.dim() != 2 or lengths.numel() != table.shape[0] or n_free.numel() != 1:
         raise KernelError(f"page_release: {lengths.numel()} lengths, a table of {tuple(table.shape)}, {n_free.numel()} counts of free pages")
+    _addresses("page_release", index, slots, table, free, n_free)
     _check(lib().sb_page_release(_i32(slots, "slots"), slots.numel(), _i32(lengths, "lengths"), _i32(table, "table"), table.shape[0],
                                  table.shape[1], _i32(free, "free"), free.numel(), _i32(n_free, "n_free"), page_size, _stream()),
            "page_release")

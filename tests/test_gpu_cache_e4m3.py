@@ -536,3 +536,52 @@ def test_refusals_in_python():
         args[i] = bad
         with pytest.raises((AssertionError, ops.KernelError)):
             ops.rope_store_e4m3(*args)
+
+
+@pytest.mark.parametrize("hd,later", [(64, 1), (64, 20), (22, 1)])
+def test_store_goes_from_the_smallest_to_the_largest_scale(hd, later):
+    """Numbers of a page whose scale grows beyond their whole range become zeros; one whose scale grows by less keeps them."""
+    cache, scales = device_cache(1, 1, hd)
+    q = torch.empty(30, 1, hd, device=DEV)
+    at = 0
+    for n, size, exponent, first in ((3, 2.0 ** -118, -126, 256.0), (later, 2.0 ** -110, -118, 1.0), (2, 2.0 ** 100, 92, 0.0)):
+        ops.rope_store_e4m3(torch.full((n, 3 * hd), size, device=DEV), 1, 1, hd, 0, None, Plan([n], [at], [[0]]), 0, cache, scales, q[:n])
+        at += n
+        # size / 2^exponent is 256, within 448 and above 224; the first token's numbers 256 * 2^(-126 - exponent)
+        assert scales.flatten().tolist() == [2.0 ** exponent] * 2
+        assert bool((cache.float()[0, :, 0, at - n:at] == 256.0).all()) and bool((cache.float()[0, :, 0, :3] == (256.0 if at == 3 else first)).all())
+
+
+def test_release_of_lengths_that_no_table_holds():
+    """Lengths up to the largest int: a slot gives back as many pages as its table has, the stack keeps to its room."""
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=DEV)                       # noqa: E731
+    lengths, table, free, n_free = i32([2 ** 31 - 1, 65, -5]), i32([[5, 6], [7, 8], [9, 10]]), i32([0, 1, -1, -1, -1]), i32([2])
+    ops.page_release(i32([0, 2, 1]), lengths, table, free, n_free)
+    # three places are left: slot 0's two pages, slot 2 has none, slot 1's first
+    assert free.tolist() == [0, 1, 5, 6, 7] and int(n_free) == 5
+    assert lengths.tolist() == [0, 0, 0] and table.tolist() == [[-1, -1], [-1, -1], [9, 10]]
+    n_free.fill_(-7)
+    lengths.copy_(i32([1, 0, 0]))
+    table[0, 0] = 3
+    ops.page_release(i32([0]), lengths, table, free, n_free)
+    assert free.tolist() == [3, 1, 5, 6, 7] and int(n_free) == 1
+
+
+def test_tables_of_lengths_that_no_table_holds():
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=DEV)                       # noqa: E731
+    t = ops.PageTables(2, 8, 8, DEV)
+    for held in (2 ** 31 - 1, 2 ** 31 - 64, -1):
+        ops.page_tables(i32([0, 1]), i32([1, 1]), i32([held, 3]), i32([[0, 1], [2, 3]]), i32([4]), i32([1]), t, 1, 2 ** 31 - 1)
+        assert int(t.status) == 2 and t.seq_row0.tolist() == [0, 0, 0] and bool((t.row_slot == -1).all())
+
+
+def test_rows_that_share_memory_are_refused():
+    cache, scales = device_cache(3, 1, 64)
+    plan = Plan([1], [3], [[0]])
+    memory = torch.zeros(512, device=DEV)
+    with pytest.raises(ops.KernelError, match="share memory"):
+        ops.rope_store_e4m3(memory[:256].view(1, 256), 2, 1, 64, 0, None, plan, 0, cache, scales, memory[128:256].view(1, 2, 64))
+    ops.rope_store_e4m3(memory[:256].view(1, 256), 2, 1, 64, 0, None, plan, 0, cache, scales, memory[256:384].view(1, 2, 64))
+    with pytest.raises(ops.KernelError, match="share memory"):
+        ops.attention_e4m3(memory[:128].view(1, 2, 64), memory[64:192].view(1, 2, 64), plan, 0, cache, scales, 2, 1, 64, 0, 0.1)
+    ops.attention_e4m3(memory[:128].view(1, 2, 64), memory[128:256].view(1, 2, 64), plan, 0, cache, scales, 2, 1, 64, 0, 0.1)
