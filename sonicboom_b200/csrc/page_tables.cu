@@ -30,8 +30,10 @@ __device__ __forceinline__ Sums up(Sums v, int o) {
   return {__shfl_up_sync(0xffffffffu, v.rows, o), __shfl_up_sync(0xffffffffu, v.total, o), __shfl_up_sync(0xffffffffu, v.taken, o)};
 }
 
-// Pages of so many tokens (0 or more, up to the largest int).
-__device__ __forceinline__ int pages_of(int tokens, int page_size) { return tokens > 0 ? (tokens - 1) / page_size + 1 : 0; }
+// Pages of so many tokens, up to the largest int; none of fewer than 0.
+__device__ __forceinline__ int pages_of(int tokens, int page_size) {
+  return (int)(((unsigned)max(tokens, 0) + (unsigned)page_size - 1u) / (unsigned)page_size);
+}
 
 // The last i with at[i] <= v, of n + 1 ascending numbers with at[0] <= v < at[n].
 __device__ __forceinline__ int owner_of(const int* at, int n, int v) {
@@ -138,7 +140,8 @@ __global__ void __launch_bounds__(TB) page_tables_kernel(const SbPageTables a) {
         if (r < n_rows) {
           s = owner_of(row0, a.n_seqs, r);
           pos = length[s] + r - row0[s];
-          where = page_of(s, pos / a.page_size) * a.page_size + pos % a.page_size;
+          const int nth = (int)((unsigned)pos / (unsigned)a.page_size);
+          where = page_of(s, nth) * a.page_size + pos - nth * a.page_size;
         }
         a.row_seq[r] = s;
         a.row_pos[r] = pos;
