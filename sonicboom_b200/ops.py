@@ -948,6 +948,8 @@ def page_tables(slots: torch.Tensor, new: torch.Tensor, lengths: torch.Tensor, t
     _check(lib().sb_page_tables(_pack_tables(
         named, brought, held, pages, stack, top, *tables._pointers, n, *shape, free.numel(), tables.page_size, tables.n_rows, tables.max_pages,
         max_new, max_len), _stream_of(index)), what)
+    if max_len != tables.max_len:                # the list is no longer than this: room that kernels need for each of its pages
+        tables.groups[0].page_ids = tables.page_ids[:tables.n_seqs * -(-max_len // tables.page_size)]
     tables.max_new, tables.max_len = max_new, max_len
     return tables
 

@@ -8,6 +8,7 @@ import torch
 
 import plain_cache_e4m3 as plain
 from sonicboom_b200 import ops
+from sonicboom_b200.cache import DevicePages
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -585,3 +586,26 @@ def test_rows_that_share_memory_are_refused():
     with pytest.raises(ops.KernelError, match="share memory"):
         ops.attention_e4m3(memory[:128].view(1, 2, 64), memory[64:192].view(1, 2, 64), plan, 0, cache, scales, 2, 1, 64, 0, 0.1)
     ops.attention_e4m3(memory[:128].view(1, 2, 64), memory[128:256].view(1, 2, 64), plan, 0, cache, scales, 2, 1, 64, 0, 0.1)
+
+
+def test_room_for_values_goes_by_the_step_and_not_by_the_pool():
+    """A prompt's attention by way of values takes room for the pages that its requests can have, not for all there are."""
+    pages = DevicePages(4, 4096, 1024, DEV)
+    tables = pages.tables(2, 300)
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=DEV)                       # noqa: E731
+    slots, new = i32([3, 1]), i32([200, 70])
+    pages.plan(slots, new, tables, 200, 256)
+    cache, scales = device_cache(16, 1, 64)
+    g = torch.Generator().manual_seed(9)
+    qkv = torch.randn(300, 4 * 64, generator=g).to(DEV)
+    q, few, values = (torch.zeros(300, 2, 64, dtype=torch.bfloat16, device=DEV) for _ in range(3))
+    ops.rope_store_e4m3(qkv, 2, 1, 64, 0, None, tables, 0, cache, scales, q)
+    ops.attention_e4m3(q, few, tables, 0, cache, scales, 2, 1, 64, 0, 0.125, kernel="few")
+    ops.attention_e4m3(q, values, tables, 0, cache, scales, 2, 1, 64, 0, 0.125, kernel="values")
+    # 8 pages of 2 * 64 * 64 values in bfloat16, their numbers, partial rows of 4 splits of 300 * 2 rows at most: under 2 MB
+    assert tables.groups[0].page_ids.numel() == 8 and sum(t.numel() for t in tables._scratch) < 2 << 20
+    # values of size 1, weights that add up to 1: the two differ by roundings of the weights (2^-8) and of the results (2^-8), times |v| < 8
+    assert float((few[:270].float() - values[:270].float()).abs().max()) <= 8 * 2.0 ** -7 and bool((values[270:] == 0).all())
+    # a longer bound gives the whole room back
+    pages.plan(slots, new, tables, 200)
+    assert tables.groups[0].page_ids.numel() == 2048
