@@ -611,7 +611,8 @@ __device__ __forceinline__ Sum sum_of_stretch(const float* row_splits, int i, in
   Sum x[STRETCH], s = {make_float4(0.0f, 0.0f, 0.0f, 0.0f), -INFINITY, 0.0f};
 #pragma unroll
   for (int u = 0; u < STRETCH; ++u) {
-    const float* src = row_splits + (size_t)min(i * STRETCH + u, n_splits - 1) * PART;
+    if (i * STRETCH + u >= n_splits) break;
+    const float* src = row_splits + (size_t)(i * STRETCH + u) * PART;
     x[u].v = __ldcg(reinterpret_cast<const float4*>(src + c));
     const float2 ml = __ldcg(reinterpret_cast<const float2*>(src + HD));
     x[u].m = ml.x;
