@@ -70,7 +70,8 @@ struct Args {
   const uint8_t* cache;                          // [page][k|v][kv head][PAGE][HD]
   const float* scales;                           // [page][k|v][kv head]
   float* scratch;                                // [row][q head][split][PART]
-  int n_q_heads, n_kv_heads, n_pages, window, n_splits;
+  int n_q_heads, n_kv_heads, group, n_pages, window, n_splits;    // group = n_q_heads / n_kv_heads
+  uint32_t by_group;                             // ceil(2^32 / group), or 0
   float scale_log2;
 };
 
@@ -78,15 +79,13 @@ struct Args {
 // less (a block's start and its partial rows).  Four, eight and sixteen pages at 28/4 heads of 128, us with the merge: one sequence of
 // 1,500 keys 7.5, 9.6, 12.8 and 64 of them 32.7, 28.9, 30.6; of 6,000 keys 7.7, 9.4, 13.1 and 92.4, 73.9, 71.6; one of 30,000
 // 17.6, 14.1, 14.7 and four of them 35.1, 28.2, 26.8.
-__host__ __device__ constexpr int split_pages(int len) {
-  return len <= 2048 ? 4 : len <= 16384 ? 8 : len <= 131072 ? 16 : len <= 524288 ? 64 : 256;
-}
+__host__ __device__ constexpr int split_shift(int len) { return len <= 2048 ? 2 : len <= 16384 ? 3 : len <= 131072 ? 4 : len <= 524288 ? 6 : 8; }
 constexpr int STRETCH = 8;                       // splits that are added up together
 long most_splits(int max_len) {
   long most = 1;
   for (long len : {2048L, 16384L, 131072L, 524288L, (long)max_len})
     if (len <= max_len) {
-      const long keys = split_pages((int)len) * PAGE, n = (len + keys - 1) / keys;
+      const long keys = (long)PAGE << split_shift((int)len), n = (len + keys - 1) / keys;
       if (n > most) most = n;
     }
   return most;
@@ -97,6 +96,7 @@ struct Seq {
   int row0, n_new, pos0, last, low, sp, split_lo, split_hi;
   bool reads;                                    // its new positions lie in its own pages
 };
+static_assert(PAGE == 1 << 6, "pages and splits by shifts");
 __device__ __forceinline__ Seq sequence(const Args& a, int b) {
   Seq s;
   s.row0 = a.seq_row0[b];
@@ -104,10 +104,11 @@ __device__ __forceinline__ Seq sequence(const Args& a, int b) {
   s.pos0 = a.seq_pos0[b];
   s.last = s.pos0 + s.n_new - 1;
   s.low = a.window > 0 ? max(0, s.pos0 - a.window + 1) : 0;
-  s.sp = split_pages(s.last + 1);
-  s.split_lo = s.low / (s.sp * PAGE);
-  s.split_hi = max(s.last, 0) / (s.sp * PAGE);
-  s.reads = s.pos0 >= 0 && s.last / PAGE < a.page_off[b + 1] - a.page_off[b] && s.split_hi < a.n_splits;
+  const int shift = split_shift(s.last + 1), last_page = max(s.last, 0) >> 6;
+  s.sp = 1 << shift;
+  s.split_lo = s.low >> (6 + shift);
+  s.split_hi = last_page >> shift;
+  s.reads = s.pos0 >= 0 && last_page < a.page_off[b + 1] - a.page_off[b] && s.split_hi < a.n_splits;
   return s;
 }
 
@@ -295,11 +296,16 @@ __global__ void __launch_bounds__(WARPS * 32, HD <= 128 && NT == 1 && sizeof(T) 
   sb_pdl_wait();
   sb_pdl_launch();
   const int split = blockIdx.x, kvh = blockIdx.y % a.n_kv_heads, row_base = blockIdx.y / a.n_kv_heads * ROWS, b = blockIdx.z;
-  const int G = a.n_q_heads / a.n_kv_heads;
+  const int G = a.group;
+  // r / G: by_group is too large by less than G / 2^32, exact while r G < 2^32 (the host sees to that)
+  auto token_of = [&](int r) { return a.by_group ? (int)__umulhi((uint32_t)r, a.by_group) : r / G; };
   const Seq sq = sequence(a, b);
   const int R = sq.n_new * G;                    // rows of this sequence and head: (new token r / G, query head r % G of the group)
   if (row_base >= R) return;
-  auto row_at = [&](int r) { return (size_t)(sq.row0 + r / G) * a.n_q_heads + kvh * G + r % G; };
+  auto row_at = [&](int r) {
+    const int token = token_of(r);
+    return (size_t)(sq.row0 + token) * a.n_q_heads + kvh * G + r - token * G;
+  };
   if (!sq.reads) {                               // zeros; no page is read
     if (split == 0)
       for (int i = tid; i < min(ROWS, R - row_base) * (HD / 4); i += WARPS * 32)
@@ -310,10 +316,10 @@ __global__ void __launch_bounds__(WARPS * 32, HD <= 128 && NT == 1 && sizeof(T) 
   const bool single = sq.split_lo == sq.split_hi;
   // the rows' positions and what they see; the last row's lowest key and the first row's position bound the pages that all rows
   // see whole
-  const int first_pos = sq.pos0 + row_base / G, last_pos = sq.pos0 + (min(row_base + ROWS, R) - 1) / G;
+  const int first_pos = sq.pos0 + token_of(row_base), last_pos = sq.pos0 + token_of(min(row_base + ROWS, R) - 1);
   auto low_of = [&](int pos) { return a.window > 0 ? max(0, pos - a.window + 1) : 0; };
   const int low = low_of(first_pos), high_low = low_of(last_pos);
-  const int tile_lo = max(split * sq.sp, low / PAGE), tile_hi = min(split * sq.sp + sq.sp - 1, last_pos / PAGE);
+  const int tile_lo = max(split * sq.sp, low >> 6), tile_hi = min(split * sq.sp + sq.sp - 1, last_pos >> 6);
   const int32_t* pages = a.page_ids + a.page_off[b];
   // Page i of this warp's (i from 0) goes to places 2 (i mod AHEAD) and the next; lane 0 asks for its tiles, every lane waits for them.
   const int n_tiles = (tile_hi - tile_lo - warp + WARPS) / WARPS;   // none or less: no page is this warp's
@@ -369,7 +375,7 @@ __global__ void __launch_bounds__(WARPS * 32, HD <= 128 && NT == 1 && sizeof(T) 
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
       const int row = row_base + 8 * n + 2 * t + r;
-      row_pos[n][r] = row < R ? sq.pos0 + row / G : -1;
+      row_pos[n][r] = row < R ? sq.pos0 + token_of(row) : -1;
       row_low[n][r] = low_of(row_pos[n][r]);
     }
   int i = 0, gave_up = 0;                        // 1: at a page's keys, 2: at its values
@@ -513,7 +519,7 @@ __global__ void __launch_bounds__(WARPS * 32, HD <= 128 && NT == 1 && sizeof(T) 
             float count[NT][HD / 16][4] = {};
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-              const int row = row_base + 8 * n + g, pos = row < R ? sq.pos0 + row / G : -1, lo = low_of(pos);
+              const int row = row_base + 8 * n + g, pos = row < R ? sq.pos0 + token_of(row) : -1, lo = low_of(pos);
 #pragma unroll
               for (int h = 0; h < 2; ++h) {
                 const int first = key0 + STEP_KEYS * sub + HALF_KEYS * h, even = first + even_key, odd = first + odd_key;
@@ -709,8 +715,10 @@ extern "C" int sb_attention_e4m3(const SbAttentionE4m3* args, cudaStream_t strea
   const size_t need = sb_attention_e4m3_scratch_bytes(x.n_rows, n_q_heads, x.max_len);
   if (need > x.scratch_bytes || (need && !x.scratch))
     SB_FAIL(SB_ERR_ARG, "%s: %zu bytes of scratch needed, %zu given", who, need, x.scratch_bytes);
+  const int group = n_q_heads / n_kv_heads;
+  const uint32_t by_group = group > 1 && (uint64_t)(rows + 15) * group < 1ull << 32 ? (uint32_t)(((1ull << 32) + group - 1) / group) : 0;
   const Args a = {x.q, x.out, x.seq_row0, x.seq_pos0, x.page_off, x.page_ids, (const uint8_t*)x.cache, x.scales, (float*)x.scratch,
-                  n_q_heads, n_kv_heads, x.n_pages, x.window, (int)n_splits, x.scale * LOG2E};
+                  n_q_heads, n_kv_heads, group, x.n_pages, x.window, (int)n_splits, by_group, x.scale * LOG2E};
   const dim3 grid((unsigned)n_splits, (unsigned)(groups * n_kv_heads), n_seqs);
   cudaError_t e = cudaSuccess;
 #if SB_HD <= 128
