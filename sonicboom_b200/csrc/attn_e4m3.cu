@@ -77,8 +77,8 @@ struct Args {
 
 // Pages of a split of a sequence of this length.  Shorter splits give few sequences enough blocks, longer ones cost many sequences
 // less (a block's start and its partial rows).  Four, eight and sixteen pages at 28/4 heads of 128, us with the merge: one sequence of
-// 1,500 keys 7.5, 9.6, 12.8 and 64 of them 32.7, 28.9, 30.6; of 6,000 keys 7.7, 9.4, 13.1 and 92.4, 73.9, 71.6; one of 30,000
-// 17.6, 14.1, 14.7 and four of them 35.1, 28.2, 26.8.
+// 1,500 keys 7.4, 9.2, 12.5 and 64 of them 31.8, 27.4, 29.1; of 6,000 keys 7.3, 9.2, 12.9 and 88.9, 72.8, 71.2; one of 30,000
+// 17.2, 13.8, 14.4 and four of them 34.3, 27.7, 26.3.
 __host__ __device__ constexpr int split_shift(int len) { return len <= 2048 ? 2 : len <= 16384 ? 3 : len <= 131072 ? 4 : len <= 524288 ? 6 : 8; }
 constexpr int STRETCH = 8;                       // splits that are added up together
 long most_splits(int max_len) {

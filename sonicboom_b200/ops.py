@@ -765,7 +765,7 @@ def _reads_pages_directly(plan, dtype, n_q_heads: int, n_kv_heads: int, head_dim
     converted again for every sixteen; or to their values, written out first, 256 rows at a time.  The first one's time grows with
     rows x keys, the second one's with the keys that a block walks alone.  In us, fitted to 1 and 8 sequences, 7 to 448 rows, 100
     to 16,000 keys, head sizes 64 and 128 (the choice is the faster one in all but near ties: 8 sequences of 112 rows over 900
-    keys 31 us and 27 us, 63 rows over 4,000 keys 47 us and 86 us, one of 448 rows over 4,000 keys 42 us and 75 us).
+    keys 30 us and 26 us, 63 rows over 4,000 keys 47 us and 86 us, one of 448 rows over 4,000 keys 41 us and 75 us).
     float32 rows do, eight at a time, as far as a grid and a few GB of partial rows go: their other way is 2.5 to 40 times slower."""
     rows, keys = plan.max_new * (n_q_heads // n_kv_heads), plan.max_len
     if rows <= 16:
