@@ -26,7 +26,8 @@ RECORDS = {
     "SbAttentionE4m3": "ppppppppp" "z" "iiiiiiiiiii" "f",
 }
 _FORMAT = {"p": "P", "z": "N", "i": "i", "f": "f"}
-RECORD_STRUCTS = {name: struct.Struct("@" + "".join(_FORMAT[c] for c in codes)) for name, codes in RECORDS.items()}
+# "0P": padded to a pointer's alignment, as a C struct is (its copy reads the padding too)
+RECORD_STRUCTS = {name: struct.Struct("@" + "".join(_FORMAT[c] for c in codes) + "0P") for name, codes in RECORDS.items()}
 pack = {name: s.pack for name, s in RECORD_STRUCTS.items()}
 
 EVERY_LIBRARY = {
