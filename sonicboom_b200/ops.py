@@ -866,8 +866,13 @@ def attention_e4m3(q: torch.Tensor, out: torch.Tensor, plan, group_index: int, c
         _attention_of_values(q, (rows, to, kept, kept_scales, row0, pos0, off, ids), plan, g, cache, n_q_heads, n_kv_heads, head_dim, window,
                              scale, index)
         return out
+    row_seq, row_pos = plan.row_seq, plan.row_pos
+    if row_seq.dtype is not _I32T or row_pos.dtype is not _I32T or not row_seq.numel() == row_pos.numel() == n:
+        raise KernelError(f"{what}: a sequence and a position in int32 for each of {n} rows, got {row_seq.dtype} {tuple(row_seq.shape)} and "
+                          f"{row_pos.dtype} {tuple(row_pos.shape)}")
+    of, at = _addresses(what, index, row_seq, row_pos)
     _check(lib().sb_attention_e4m3_plain(
-        rows, to, _code(dtype), n, _i32(plan.row_seq, "row_seq"), _i32(plan.row_pos, "row_pos"), off, ids, g.page_size, kept, kept_scales,
+        rows, to, _code(dtype), n, of, at, off, ids, g.page_size, kept, kept_scales,
         cache.shape[0], n_q_heads, n_kv_heads, head_dim, window, scale, _stream_of(index)), "attention_e4m3 (plain kernel)")
     return out
 

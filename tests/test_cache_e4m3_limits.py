@@ -13,3 +13,70 @@ def test_a_packed_record_is_as_long_as_its_struct(name):
     of = {"p": ctypes.c_void_p, "z": ctypes.c_size_t, "i": ctypes.c_int, "f": ctypes.c_float}
     struct = type(name, (ctypes.Structure,), {"_fields_": [(f"m{i}", of[c]) for i, c in enumerate(abi.RECORDS[name])]})
     assert len(abi.pack[name](*[0] * len(abi.RECORDS[name]))) == abi.RECORD_STRUCTS[name].size == ctypes.sizeof(struct)
+
+
+# ------------------------------------------------------------------------------------------------ calls that a fake library records
+class Recorder:
+    """A library whose entry points note their arguments and succeed."""
+
+    def __init__(self):
+        self.calls = []
+
+    def __getattr__(self, name):
+        def entry(*args):
+            self.calls.append((name, args))
+            return 0
+        return entry
+
+
+@pytest.fixture
+def recorder(monkeypatch):
+    """The operators on host tensors, as far as their calls of the library: nothing is computed."""
+    r = Recorder()
+    monkeypatch.setattr(ops, "_device_of", lambda t, what: -1)
+    monkeypatch.setattr(ops, "_stream_of", lambda index: 0)
+    monkeypatch.setattr(ops, "_sm_count", lambda index: 148)
+    monkeypatch.setattr(ops, "lib", lambda: r)
+    monkeypatch.setattr(ops, "attention_lib", lambda head_dim: r)
+    monkeypatch.setattr(ops, "_attn_counters", lambda n, device: torch.zeros(n, dtype=torch.int32))
+    return r
+
+
+def i32(values):
+    return torch.tensor(values, dtype=torch.int32)
+
+
+class Plan:
+    def __init__(self, new, pos0, lists):
+        self.n_seqs, self.n_rows, self.max_new, self.max_len = len(new), sum(new), max(new), max(p + n for p, n in zip(pos0, new))
+        row0, off = [0], [0]
+        for n, pages in zip(new, lists):
+            row0.append(row0[-1] + n)
+            off.append(off[-1] + len(pages))
+        self.seq_row0, self.seq_pos0 = i32(row0), i32(pos0)
+        self.row_seq = i32([i for i, n in enumerate(new) for _ in range(n)])
+        self.row_pos = i32([p + j for p, n in zip(pos0, new) for j in range(n)])
+        self.groups = [ops.TableGroup(i32(off), i32([p for pages in lists for p in pages]), 64)]
+
+    def scratch(self, nbytes, device):
+        return torch.empty(nbytes, dtype=torch.uint8) if nbytes else None
+
+
+def attend(plan, hq=4, hkv=2, hd=64, dtype=torch.bfloat16, kernel="auto", window=0):
+    cache = torch.zeros(4, 2, hkv, 64, hd, dtype=torch.uint8).view(torch.float8_e4m3fn)
+    q, out = (torch.zeros(plan.n_rows, hq, hd, dtype=dtype) for _ in range(2))
+    return ops.attention_e4m3(q, out, plan, 0, cache, torch.ones(4, 2, hkv), hq, hkv, hd, window, 0.125, kernel)
+
+
+@pytest.mark.parametrize("field", ["row_seq", "row_pos"])
+def test_the_plain_kernels_row_arrays_are_checked(recorder, field):
+    """It reads a sequence and a position for every row."""
+    plan = Plan([1, 2], [70, 5], [[0, 1], [2]])
+    attend(plan, kernel="plain")
+    assert [name for name, _ in recorder.calls] == ["sb_attention_e4m3_plain"]
+    good = getattr(plan, field)
+    for bad in (good[:2], good.long(), torch.stack([good, good])):
+        setattr(plan, field, bad)
+        with pytest.raises(ops.KernelError, match="attention_e4m3"):
+            attend(plan, kernel="plain")
+    assert len(recorder.calls) == 1
