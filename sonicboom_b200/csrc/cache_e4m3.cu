@@ -223,8 +223,7 @@ __global__ void __launch_bounds__(THREADS) store_many_kernel(const SbStoreE4m3 a
 // that lie wholly before the window are left out.  A sequence whose positions have no pages gets rows of zeros in `out`, which
 // the attention behind this kernel leaves alone.  One block a page and head, 16 bytes out a thread and step
 // (8 bytes in for bfloat16: with 16 in and 32 out a thread, 16,512 tokens took 24 us instead of 10); bound by memory (1 byte in, 2 or
-// 4 out a value) or, at few pages, by its start.  It lets its successor start at its end only: that may read `numbers` ahead of its own
-// wait, as attention of few rows does.
+// 4 out a value) or, at few pages, by its start.  What attends to the values waits for this kernel before it reads any of them.
 constexpr int VALUES_THREADS = 128;
 
 // Numbers times a scale, 16 bytes of results: eight of bfloat16, four of float32 (or of bfloat16, 8 bytes).
@@ -263,10 +262,7 @@ values_kernel(const int32_t* seq_row0, const int32_t* seq_pos0, const int32_t* p
   }
   const int start = i * page_size, low = window > 0 ? max(0, pos0 - window + 1) : 0;
   if (start >= len || first + i >= n_list) return;
-  if (head == 0 && tid == 0) {
-    numbers[first + i] = first + i;
-    __threadfence();                             // a successor may read it ahead of its wait, once this grid's blocks are done
-  }
+  if (head == 0 && tid == 0) numbers[first + i] = first + i;
   if (start + page_size <= low) return;
   const int page = min(max(page_ids[first + i], 0), n_pages - 1);
   const size_t block = (size_t)page * gridDim.y + head;

@@ -785,11 +785,6 @@ def _e4m3_scratch_bytes(head_dim: int, n_rows: int, n_q_heads: int, max_len: int
     return int(attention_lib(head_dim).sb_attention_e4m3_scratch_bytes(n_rows, n_q_heads, max_len))
 
 
-@functools.lru_cache(maxsize=1024)
-def _attention_scratch_bytes(head_dim: int, n_rows: int, n_q_heads: int, n_kv_heads: int, max_new: int, max_len: int) -> int:
-    return int(attention_lib(head_dim).sb_attention_scratch_bytes(n_rows, n_q_heads, n_kv_heads, max_new, max_len))
-
-
 def _attention_of_values(q, addresses, plan, g, cache, n_q_heads, n_kv_heads, head_dim, window, scale, index):
     """`attention_e4m3` by way of the step's pages as values of q's type, one after another in scratch memory; what `attention` does
     over them, with the addresses at hand (a call takes 18 us instead of 38 where the GPU takes less)."""
@@ -799,9 +794,8 @@ def _attention_of_values(q, addresses, plan, g, cache, n_q_heads, n_kv_heads, he
     bf16 = q.dtype is torch.bfloat16
     n_values = n_list * 2 * n_kv_heads * g.page_size * head_dim * (2 if bf16 else 4) + 255 & ~255
     n_numbers = 4 * n_list + 255 & ~255
-    need = _attention_scratch_bytes(head_dim, n, n_q_heads, n_kv_heads, plan.max_new, plan.max_len) if bf16 else 0
-    values = plan.scratch(n_values + n_numbers + need, q.device).data_ptr()
-    numbers, partial = values + n_values, values + n_values + n_numbers
+    values = plan.scratch(n_values + n_numbers, q.device).data_ptr()
+    numbers = values + n_values
     _check(l.sb_cache_e4m3_values(
         row0, pos0, plan.n_seqs, plan.max_len, off, ids, n_list, g.page_size, kept, kept_scales, cache.shape[0], n_q_heads, n_kv_heads,
         head_dim, window, values, dtype, numbers, to, stream), "attention_e4m3 (values)")
@@ -810,11 +804,12 @@ def _attention_of_values(q, addresses, plan, g, cache, n_q_heads, n_kv_heads, he
             rows, to, n, plan.n_seqs, plan.max_new, plan.max_len, row0, pos0, off, numbers, g.page_size, values, n_list, n_q_heads, n_kv_heads,
             head_dim, window, scale, None, 0.0, 0, None, 0, _sm_count(index), stream), "attention_e4m3 (float32 values)")
         return
-    al, counters = attention_lib(head_dim), _attn_counters(plan.n_seqs * n_kv_heads, q.device)
+    # `attention` of few rows asks for pages of older tokens ahead of its wait for the kernel before it, which has only just written
+    # these: a bound of more rows than it takes leaves the step to the kernels that wait first (they need no scratch memory)
+    al, max_new = attention_lib(head_dim), max(plan.max_new, DECODE_ATTENTION_ROWS // (n_q_heads // n_kv_heads) + 1)
     rc = al.sb_attention(
-        rows, to, n, plan.n_seqs, plan.max_new, row0, pos0, off, numbers, g.page_size, values, n_q_heads, n_kv_heads, head_dim, window, scale,
-        partial if need else None, need, counters.data_ptr(), counters.numel(), plan.max_len, n_list, _sm_count(index), None, 0, None, 0.0, 0,
-        None, 0, stream)
+        rows, to, n, plan.n_seqs, max_new, row0, pos0, off, numbers, g.page_size, values, n_q_heads, n_kv_heads, head_dim, window, scale,
+        None, 0, None, 0, plan.max_len, n_list, _sm_count(index), None, 0, None, 0.0, 0, None, 0, stream)
     if rc != 0:
         raise KernelError(f"{what}: {al.sb_last_error().decode()}")
     LAUNCHES += int(al.sb_attention_last_launches())

@@ -80,3 +80,13 @@ def test_the_plain_kernels_row_arrays_are_checked(recorder, field):
         with pytest.raises(ops.KernelError, match="attention_e4m3"):
             attend(plan, kernel="plain")
     assert len(recorder.calls) == 1
+
+
+@pytest.mark.parametrize("hq,hkv,new", [(4, 2, [1, 1]), (28, 4, [2]), (16, 1, [1]), (17, 1, [1]), (4, 2, [40, 3])])
+def test_values_are_read_by_kernels_that_wait_for_them(recorder, hq, hkv, new):
+    """The kernels of `attention` for few rows read old pages ahead of their wait for the kernel before them; here that one has
+    just written them.  So the call asks for more rows a key/value head than those kernels take."""
+    plan = Plan(new, [70] * len(new), [[0, 1], [2, 3]][:len(new)])
+    attend(plan, hq, hkv, kernel="values")
+    (args,) = [args for name, args in recorder.calls if name == "sb_attention"]
+    assert args[4] >= plan.max_new and args[4] * (hq // hkv) > ops.DECODE_ATTENTION_ROWS
