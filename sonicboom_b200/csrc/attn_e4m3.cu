@@ -280,12 +280,11 @@ __global__ void __launch_bounds__(WARPS * 32, HD <= 128 && NT == 1 && sizeof(T) 
   float(*part)[ROWS][PART] = reinterpret_cast<float(*)[ROWS][PART]>(tiles);
   __shared__ float stat_m[WARPS][ROWS], stat_l[WARPS][ROWS], stat_n[WARPS][ROWS];
   __shared__ __align__(8) uint64_t landed[WARPS][2 * AHEAD];
-  __shared__ int failed;
+  __shared__ int stopped[WARPS];                 // what each warp gave up at, or 0
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   const unsigned char* const my_tiles = tiles + warp * (2 * AHEAD * TILE_SMEM);
   const uint32_t ring = (uint32_t)__cvta_generic_to_shared(my_tiles);
   const uint32_t bars = (uint32_t)__cvta_generic_to_shared(landed[warp]);
-  if (tid == 0) failed = 0;
   if (lane == 0) {                               // barriers and tiles of a warp's own
 #pragma unroll
     for (int i = 0; i < 2 * AHEAD; ++i) mbar_init(bars + 8 * i, 1);
@@ -545,12 +544,11 @@ __global__ void __launch_bounds__(WARPS * 32, HD <= 128 && NT == 1 && sizeof(T) 
     k_scale = next_k;
     v_scale = next_v;
   }
-  if (gave_up) {                                 // nothing is written; the block's memory outlives its copies
+  if (gave_up)                                   // nothing is written; the block's memory outlives its copies
     for (int j = i; j < min(n_tiles, i + AHEAD + 1); ++j)
       for (int v = 0; v < 2; ++v)
         if (j < i + AHEAD || (v == 0 && gave_up == 2)) mbar_wait(bars + 8 * (2 * (j % AHEAD) + v), j / AHEAD & 1, 33);
-    failed = 1;
-  }
+  if (lane == 0) stopped[warp] = gave_up;
 
   // the warps' partial results, over the tiles
   __syncthreads();
@@ -573,6 +571,9 @@ __global__ void __launch_bounds__(WARPS * 32, HD <= 128 && NT == 1 && sizeof(T) 
   }
   __syncthreads();
   // merged in the warps' order: o relative to the largest score, that score, the weights' sum
+  int failed = 0;
+#pragma unroll
+  for (int w = 0; w < WARPS; ++w) failed |= stopped[w];
   const int n_items = failed ? 0 : min(ROWS, R - row_base) * (HD / 4);
   for (int j = tid; j < n_items; j += WARPS * 32) {
     const int row = j / (HD / 4), c = 4 * (j % (HD / 4));
