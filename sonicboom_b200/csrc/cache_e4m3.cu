@@ -220,8 +220,9 @@ __global__ void __launch_bounds__(THREADS) store_many_kernel(const SbStoreE4m3 a
 // The pages of a step's sequences as values in bfloat16 or float32, one after another as the plan lists them: [place in
 // page_ids][k|v][head][position][hd], with `numbers` for the page list that says so.  Exact in either type (a number has four bits, the scale is a power of two).  What no row of
 // the step sees (positions behind a sequence's end, before its first row's window) becomes 0, whatever the page holds there; pages
-// that lie wholly before the window are left out.  A sequence whose positions have no pages gets rows of zeros in `out`, which
-// the attention behind this kernel leaves alone.  One block a page and head, 16 bytes out a thread and step
+// that lie wholly before the window are left out.  A sequence whose list ends before its last row gets rows of zeros in `out`, which
+// the attention of bfloat16 rows behind this kernel leaves alone; that of float32 rows goes row by row, and finds that the pages
+// there are have no number: their keys and values count as zeros.  One block a page and head, 16 bytes out a thread and step
 // (8 bytes in for bfloat16: with 16 in and 32 out a thread, 16,512 tokens took 24 us instead of 10); bound by memory (1 byte in, 2 or
 // 4 out a value) or, at few pages, by its start.  What attends to the values waits for this kernel before it reads any of them.
 constexpr int VALUES_THREADS = 128;
@@ -258,6 +259,7 @@ values_kernel(const int32_t* seq_row0, const int32_t* seq_pos0, const int32_t* p
     for (size_t at = ((size_t)i * gridDim.y + head) * VALUES_THREADS + tid; at < (size_t)n_new * out_width;
          at += (size_t)gridDim.x * gridDim.y * VALUES_THREADS)
       out[(size_t)row0 * out_width + at] = sb_from_f32<T>(0.0f);
+    if (i < n_own && first + i < n_list && head == 0 && tid == 0) numbers[first + i] = -1;
     return;
   }
   const int start = i * page_size, low = window > 0 ? max(0, pos0 - window + 1) : 0;
@@ -302,7 +304,7 @@ template <typename TQ>
 __global__ void __launch_bounds__(PLAIN_THREADS)
 attention_kernel(const TQ* q, TQ* out, const int32_t* row_seq, const int32_t* row_pos, const int32_t* page_off, const int32_t* page_ids,
                  int page_size, const uint8_t* cache, const float* scales, int n_pages, int n_q_heads, int n_kv_heads, int hd, int window,
-                 float scale) {
+                 float scale, int n_rows) {
   __shared__ float qs[PLAIN_MAX_HD], scores[PLAIN_CHUNK], shared[4];
   sb_pdl_launch();
   sb_pdl_wait();
@@ -310,8 +312,15 @@ attention_kernel(const TQ* q, TQ* out, const int32_t* row_seq, const int32_t* ro
   const int kvh = h / (n_q_heads / n_kv_heads), pos = row_pos[t], seq = row_seq[t];
   TQ* dst = out + ((size_t)t * n_q_heads + h) * hd;
   if (pos < 0) return;                           // a row behind the last sequence: left as it is
+  // The sequence's last row: its rows follow one another, with another sequence's or rows of none behind them.
+  int last = t, end = n_rows;
+  while (end - last > 1) {
+    const int mid = (last + end) >> 1;
+    if (row_seq[mid] == seq && row_pos[mid] > pos) last = mid;
+    else end = mid;
+  }
   const int n_own = page_off[seq + 1] - page_off[seq];
-  if (pos / page_size >= n_own) {                // a position without a page: zeros, nothing is read
+  if (row_pos[last] / page_size >= n_own) {      // the list ends before that one: zeros, nothing is read
     for (int d = tid; d < hd; d += PLAIN_THREADS) dst[d] = sb_from_f32<TQ>(0.0f);
     return;
   }
@@ -473,7 +482,7 @@ extern "C" int sb_attention_e4m3_plain(const void* q, void* out, int act_dtype, 
   SB_DISPATCH_DTYPE(act_dtype, TQ, {
     sb_launch<SB_K_OTHER>(attention_kernel<TQ>, dim3(n_rows, n_q_heads), dim3(PLAIN_THREADS), 0, stream, (const TQ*)q, (TQ*)out, row_seq,
                           row_pos, page_off, page_ids, page_size, (const uint8_t*)cache, scales, n_pages, n_q_heads, n_kv_heads, hd, window,
-                          scale);
+                          scale, n_rows);
   });
   SB_CHECK_LAUNCH(who);
   return SB_OK;

@@ -509,13 +509,15 @@ typedef struct SbStoreE4m3 {
 } SbStoreE4m3;
 int sb_rope_store_e4m3(const SbStoreE4m3* args, sb_stream_t stream);
 /* The pages of a step's sequences as values (exactly), one after another as page_ids [n_list] lists them, [k|v][kv head][position]
- * [hd] each, with the page list numbers [n_list] that says so; 0 at positions that no row of the step sees.  Pages wholly before the window are left out.  Sequences whose positions
- * have no pages get zeros in out [rows][n_q_heads * hd], of the values' dtype: what attends to the values leaves them alone. */
+ * [hd] each, with the page list numbers [n_list] that says so; 0 at positions that no row of the step sees.  Pages wholly before the window are left out.  A sequence whose list ends
+ * before its last row gets zeros in out [rows][n_q_heads * hd], of the values' dtype, and -1 as its pages' numbers: what attends to the
+ * values leaves such rows alone, or finds nothing but zeros. */
 int sb_cache_e4m3_values(const int32_t* seq_row0, const int32_t* seq_pos0, int n_seqs, int max_len, const int32_t* page_off,
                          const int32_t* page_ids, int n_list, int page_size, const void* cache, const float* scales, int n_pages,
                          int n_q_heads, int n_kv_heads, int hd, int window, void* values, int dtype, int32_t* numbers, void* out,
                          sb_stream_t stream);
-/* sb_attention_plain over that cache: float32 arithmetic, any head size up to 1024; a row with a negative position is left as it is. */
+/* sb_attention_plain over that cache: float32 arithmetic, any head size up to 1024; a row with a negative position is left as it is,
+ * rows of a sequence whose list ends before its last row become zeros. */
 int sb_attention_e4m3_plain(const void* q, void* out, int act_dtype, int n_rows, const int32_t* row_seq, const int32_t* row_pos,
                             const int32_t* page_off, const int32_t* page_ids, int page_size, const void* cache, const float* scales,
                             int n_pages, int n_q_heads, int n_kv_heads, int hd, int window, float scale, sb_stream_t stream);

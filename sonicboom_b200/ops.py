@@ -819,7 +819,7 @@ def attention_e4m3(q: torch.Tensor, out: torch.Tensor, plan, group_index: int, c
                    n_q_heads: int, n_kv_heads: int, head_dim: int, window: int, scale: float, kernel: str = "auto") -> torch.Tensor:
     """`attention` of the step's rows over a cache held in 8 bits (see `rope_store_e4m3`): causal, grouped queries, with `window`
     n > 0 only the last n keys.  q and out bfloat16 or float32, of one dtype.  Rows behind the plan's last sequence are left as
-    they are; a sequence whose positions have no pages gets zeros.
+    they are; a sequence whose page list ends before its last new token gets zeros (of queries that are finite).
 
     Head sizes in steps of 16 up to 256 with pages of 64 keys run on tensor cores (built for the head size at first use): "few"
     reads the pages as they are, float32 rows and weights as two halves each; bfloat16 rows in such numbers that this is slower

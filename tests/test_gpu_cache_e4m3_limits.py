@@ -1,0 +1,41 @@
+"""The 8-bit cache's kernels at the limits of what their calls say: lists that end too early, tokens that were taken back, scales far
+apart, plans made on the device."""
+import pytest
+import torch
+
+import plain_cache_e4m3 as plain
+from sonicboom_b200 import ops
+from test_gpu_cache_e4m3 import DEV, Plan
+
+pytestmark = pytest.mark.gpu
+
+
+def ones(n_pages, hkv, page, hd):
+    return torch.ones(n_pages, 2, hkv, page, hd, device=DEV).to(torch.float8_e4m3fn), torch.ones(n_pages, 2, hkv, device=DEV)
+
+
+@pytest.mark.parametrize("kernel,dtype,hd,page", [
+    ("few", torch.bfloat16, 64, 64), ("few", torch.float32, 128, 64), ("values", torch.bfloat16, 64, 64), ("values", torch.bfloat16, 48, 64),
+    ("values", torch.float32, 64, 64), ("values", torch.float32, 24, 64), ("values", torch.float32, 24, 16), ("plain", torch.bfloat16, 64, 64),
+    ("plain", torch.float32, 22, 16)])
+@pytest.mark.parametrize("n", [10, 1])
+def test_a_sequence_whose_list_ends_among_its_new_rows_gets_zeros(kernel, dtype, hd, page, n):
+    """All its rows, those before the list's end too, whatever kernel runs and whatever an earlier call left in scratch memory."""
+    hq, hkv = 4, 2
+    cache, scales = ones(4, hkv, page, hd)
+    pos0 = page - 4
+    for short in (False, True):                                                 # the first call leaves pages and numbers behind
+        lists = [[0], [2, 3, 1]] if short and n > 1 else [[0, 1], [2, 3]]
+        plan = Plan([n, 2], [pos0 if n > 1 else (2 * page if short else pos0), 5], lists)
+        if short:
+            plan._scratch = scratch
+        plan.groups[0].page_size = page
+        out = torch.full((n + 2, hq * hd), 5.0, dtype=dtype, device=DEV)
+        ops.attention_e4m3(torch.ones(n + 2, hq, hd, dtype=dtype, device=DEV), out, plan, 0, cache, scales, hq, hkv, hd, 0, 0.1, kernel)
+        scratch = plan._scratch
+        # keys and values are ones: weights that add up to 1 give 1, to the roundings of at most 74 weights and of the result
+        assert float((out[n:].float() - 1).abs().max()) <= 2.0 ** -7
+        if short:
+            assert bool((out[:n] == 0).all())
+        else:
+            assert float((out[:n].float() - 1).abs().max()) <= 2.0 ** -7
