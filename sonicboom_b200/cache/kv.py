@@ -213,12 +213,18 @@ class Cache:
         """Cuts a sequence back to its first `new_len` tokens (prefix reuse).  Returns False,
         changing nothing, when a windowed group has already given back pages that the shorter
         sequence would read again, or when the model keeps fixed-size state per sequence (it
-        was advanced by the tokens that would be cut)."""
+        was advanced by the tokens that would be cut).
+
+        In a cache held in 8 bits a page's scale, and what of its older numbers is left, go back to all tokens that
+        were written to it.  So a sequence that is cut there keeps whole pages only: its length afterwards is
+        `new_len` or the end of the page before, and tokens are fed from `length(slot)` on."""
         rec = self._record(slot)
         if not 0 <= new_len <= rec.length:
             raise CacheError(f"slot {slot}: cannot truncate from {rec.length} to {new_len}")
         if self.state and new_len < rec.length:
             return False         # fixed-size state has moved on with the tokens and cannot go back
+        if new_len < rec.length and any(g.scales is not None for g in self.groups):
+            new_len -= new_len % self.page_size
         keep = (new_len + self.page_size - 1) // self.page_size
         for g, pages in zip(self.groups, rec.pages):
             first_seen = g.need.first_read(new_len) // self.page_size

@@ -91,7 +91,8 @@ class Session:
 
     def prefill(self, tokens) -> int:
         """`boom_llm_prefill`: sets the prompt.  Returns how many leading tokens were reused
-        from the cache of the previous prompt; the last prompt token is always processed."""
+        from the cache of the previous prompt; the last prompt token is always processed.  Over a cache in 8 bits
+        those of them that lie behind the last whole page are processed again (`Cache.truncate` says why)."""
         tokens = [int(t) for t in tokens]
         if not tokens:
             raise ValueError("prefill needs a non-empty prompt")
@@ -106,14 +107,14 @@ class Session:
                     break
                 common += 1
             reused = min(common, len(tokens) - 1)
-            if not self.engine.cache.truncate(self.slot, reused):
+            if not self.engine.cache.truncate(self.slot, reused) or self.engine.length(self.slot) == 0:
                 reused = 0
         if self.slot is not None and reused == 0:
             self.engine.close(self.slot)
             self.slot = None
         if self.slot is None:
             self.slot = self.engine.open()
-        rest = tokens[reused:]
+        rest = tokens[self.engine.length(self.slot):]
         self._logits = self.engine.step([(self.slot, rest, [len(rest) - 1])])
         self._pending = None
         self.tokens = tokens

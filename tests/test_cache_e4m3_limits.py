@@ -90,3 +90,27 @@ def test_values_are_read_by_kernels_that_wait_for_them(recorder, hq, hkv, new):
     attend(plan, hq, hkv, kernel="values")
     (args,) = [args for name, args in recorder.calls if name == "sb_attention"]
     assert args[4] >= plan.max_new and args[4] * (hq // hkv) > ops.DECODE_ATTENTION_ROWS
+
+
+# ------------------------------------------------------------------------------------------------ tokens that are taken back
+def test_a_cache_in_8_bits_goes_back_to_whole_pages():
+    """What is left of a page's numbers goes back to all tokens that were written to it, the cut ones too."""
+    from sonicboom_b200.cache import Cache, KVNeed
+    from sonicboom_b200.cache.kv import E4M3
+
+    def cut(kv_dtype, *lengths, window=0, held=300):
+        c = Cache([KVNeed(1, 16), KVNeed(1, 16, window)], [None] * 2, 640, torch.bfloat16, "cpu", kv_dtype=kv_dtype)
+        slot = c.open()
+        c.reserve(slot, held)
+        c.advance(slot, held)
+        done = [c.truncate(slot, n) for n in lengths]
+        c.check()
+        return done, c.length(slot), len(c.page_list(slot, 0))
+
+    assert cut(E4M3, 300) == ([True], 300, 5)                    # nothing is cut
+    assert cut(E4M3, 299) == ([True], 256, 4) and cut(E4M3, 256) == ([True], 256, 4)
+    assert cut(E4M3, 299, 256, 200, 63) == ([True] * 4, 0, 0)
+    assert cut(None, 299) == ([True], 299, 5) and cut(None, 63) == ([True], 63, 1)
+    # a window of 40 at 300 tokens has given the pages before 261 back: 299 goes back to 256, whose next token reads 217
+    assert cut(E4M3, 299, window=40) == ([False], 300, 5)
+    assert cut(E4M3, 300, window=40) == ([True], 300, 5) and cut(None, 299, window=40) == ([True], 299, 5)

@@ -39,3 +39,31 @@ def test_a_sequence_whose_list_ends_among_its_new_rows_gets_zeros(kernel, dtype,
             assert bool((out[:n] == 0).all())
         else:
             assert float((out[:n].float() - 1).abs().max()) <= 2.0 ** -7
+
+
+# ------------------------------------------------------------------------------------------------ tokens that are taken back
+def test_a_prompt_that_goes_on_in_a_cut_page_is_as_a_fresh_one(model_dirs):
+    """The page as a token far larger than the others would have left it, which is then cut away: its scale 2^20 times as large, the
+    older numbers gone."""
+    import plain_model as pm
+    from conftest import prompts_for
+    from sonicboom_b200 import llm
+    from test_gpu_engine_e4m3 import F32_TOL
+    model = llm.model_load(model_dirs["B"], dtype="float32")
+    p = prompts_for("B", [90], seed=6)[0]
+    sessions = [llm.session_new(model, 200, cache_dtype="e4m3") for _ in range(2)]
+    sessions[0].prefill(p)
+    g = sessions[0].engine.cache.groups[0]
+    page = sessions[0].engine.cache.page_list(sessions[0].slot, 0)[1]
+    g.scales[:, page] *= 2.0 ** 20
+    g.storage.view(torch.uint8)[:, page] = 0
+    logits, scales = [], []
+    for s in sessions:
+        s.prefill(p[:80] + p[:9])
+        logits.append(s._logits.cpu())
+        scales.append([s.engine.cache.groups[0].scales[:, i].cpu() for i in s.engine.cache.page_list(s.slot, 0)])
+        assert s.engine.length(s.slot) == 89
+        s.free()
+    assert pm.rel_err(logits[0], logits[1]) < F32_TOL
+    # a largest number within 2^-20 of a border would make a step of 2; none of these does
+    assert all(torch.equal(a, b) for a, b in zip(*scales)) and len(scales[0]) == 2
