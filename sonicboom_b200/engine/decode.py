@@ -49,7 +49,7 @@ class DecodePlan:
         self.seq_slot = torch.tensor(slots, dtype=torch.int32, device=device)
         self.want_rows = self.row_seq
         self.groups = []
-        self.max_len = 0
+        self.max_len, self.first_without_page = 0, [0] * n
         for gi in range(len(cache.groups)):
             lists = [cache.page_list(s, gi) for s in slots]
             off = np.zeros(n + 1, dtype=np.int32)
@@ -57,6 +57,7 @@ class DecodePlan:
             ids = np.asarray([p for l in lists for p in l], dtype=np.int32)
             self.groups.append(GroupPlan(torch.from_numpy(off).to(device),
                                          torch.from_numpy(ids).to(device), cache.page_size))
+            self.first_without_page = [max(at, len(l) * cache.page_size) for at, l in zip(self.first_without_page, lists)]
             self.max_len = max(self.max_len, max(len(l) for l in lists) * cache.page_size)
         self._scratch = None
 
@@ -105,6 +106,7 @@ class DecodeLoop:
         self.host_out = torch.zeros(n, dtype=torch.int32).pin_memory()
         self.h2d_bytes_per_step = self.d2h_bytes_per_step = 4 * n
         self.graph = None
+        self.parks = any(g.scales is not None for g in cache.groups)
         before = ops.LAUNCHES
         # One eager run first: it builds what is built lazily and sets kernel attributes, which
         # cannot happen inside a capture.  It must leave the sequences as it found them: the
@@ -142,8 +144,13 @@ class DecodeLoop:
 
     def retire(self, row: int) -> None:
         """Row `row` has finished: it stays in the captured batch as a row nobody reads, inside
-        its own pages, and `close` records only the tokens it was fed while live."""
+        its own pages, and `close` records only the tokens it was fed while live.  Over a cache held in 8 bits a token
+        of no meaning could still change the scale of the last page that counts, and its numbers with it: there the
+        row moves on to a position without a page, where nothing is written."""
         self.live[row] = False
+        if self.parks:
+            for t in (self.plan.row_pos, self.plan.row_last):
+                t[row:row + 1].fill_(self.plan.first_without_page[row])
 
     def _replay(self) -> None:
         for i, (ok, fed, b) in enumerate(zip(self.live, self.fed, self.budgets)):

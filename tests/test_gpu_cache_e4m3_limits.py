@@ -67,3 +67,31 @@ def test_a_prompt_that_goes_on_in_a_cut_page_is_as_a_fresh_one(model_dirs):
     assert pm.rel_err(logits[0], logits[1]) < F32_TOL
     # a largest number within 2^-20 of a border would make a step of 2; none of these does
     assert all(torch.equal(a, b) for a, b in zip(*scales)) and len(scales[0]) == 2
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+def test_a_retired_row_leaves_its_pages_alone(model_dirs, dtype):
+    """The captured loop goes on for another row: the retired one's pages and scales stay, also where its last page is full or its
+    budget is used up, and the sequence goes on from there as if nothing had been."""
+    from conftest import prompts_for
+    from sonicboom_b200.sampling import Sampling
+    from test_gpu_engine_e4m3 import engine
+    eng = engine(model_dirs, "B", dtype)
+    slots, lengths, budgets = [eng.open() for _ in range(4)], [70, 61, 5, 9], [12, 3, 4, 30]
+    eng.step([(s, p, [len(p) - 1]) for s, p in zip(slots, prompts_for("B", lengths, seed=3))])
+    loop = eng.decode_loop(slots, budgets, [Sampling().checked()] * 4)
+    tokens = [1, 2, 3, 4]
+    for _ in range(3):                                                          # 73, 64 (a whole page, its budget used up) and 8 tokens
+        tokens = loop.step_host(tokens)
+    g = eng.cache.groups[0]
+    before = g.storage.view(torch.uint8).clone(), g.scales.clone()
+    for row in range(3):
+        loop.retire(row)
+    for _ in range(20):
+        tokens = loop.step_host([7, 8, 9, tokens[3]])
+    for i in range(3):
+        pages = [p for p in eng.cache.page_list(slots[i], 0)]
+        assert torch.equal(before[0][:, pages], g.storage.view(torch.uint8)[:, pages]) and torch.equal(before[1][:, pages], g.scales[:, pages])
+    assert all(0 <= t for t in tokens[3:])
+    loop.close()
+    assert [eng.length(s) for s in slots] == [73, 64, 8, 32]
