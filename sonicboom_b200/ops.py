@@ -904,11 +904,13 @@ class PageTables:
 
     def scratch(self, nbytes: int, device):
         """Scratch memory shared by the step's kernels (made on first use, another one when more is asked for); None when nothing is.
-        The older ones stay: a graph that was captured with them may run again."""
+        The older ones stay: a graph that was captured with them may run again.  Each is at least twice the one before, so that
+        all of them together are less than four times what was asked for, however often a growing step asks for a little more."""
         if nbytes <= 0:
             return None
         if not self._scratch or self._scratch[-1].numel() < nbytes:
-            self._scratch.append(torch.empty(nbytes, dtype=torch.uint8, device=device))
+            size = max(nbytes, 2 * self._scratch[-1].numel()) if self._scratch else nbytes
+            self._scratch.append(torch.empty(size, dtype=torch.uint8, device=device))
         return self._scratch[-1]
 
     def check(self) -> None:

@@ -114,3 +114,14 @@ def test_a_cache_in_8_bits_goes_back_to_whole_pages():
     # a window of 40 at 300 tokens has given the pages before 261 back: 299 goes back to 256, whose next token reads 217
     assert cut(E4M3, 299, window=40) == ([False], 300, 5)
     assert cut(E4M3, 300, window=40) == ([True], 300, 5) and cut(None, 299, window=40) == ([True], 299, 5)
+
+
+def test_scratch_memory_of_tables_that_grow_step_by_step():
+    """Every buffer stays for the graphs that know it; together they are bounded by what is needed."""
+    t = ops.PageTables(1, 4, 4, "cpu")
+    first = t.scratch(100, "cpu")
+    for n in range(100, 20000, 7):
+        got = t.scratch(n, "cpu")
+        assert got.numel() >= n and sum(b.numel() for b in t._scratch) < 4 * n
+        assert t.scratch(n // 2, "cpu") is got
+    assert t._scratch[0] is first and t.scratch(0, "cpu") is None and len(t._scratch) <= 9
