@@ -117,6 +117,7 @@ CORE = {
     "sb_cache_e4m3_values": ("i", "ppiippiippiiiiipipps"),
     "sb_attention_e4m3_plain": ("i", "ppiippppippiiiiifs"),
     "sb_page_tables": ("i", "ps"),
+    "sb_page_tables_settle": ("i", "s"),
     "sb_page_advance": ("i", "ppipipips"),
     "sb_page_release": ("i", "pippiipipis"),
     "sb_sample_params_size": ("i", ""),

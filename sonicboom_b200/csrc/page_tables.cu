@@ -158,6 +158,9 @@ __global__ void __launch_bounds__(TB) page_tables_kernel(const SbPageTables a) {
   }
 }
 
+// Nothing: see sb_page_tables_settle.
+__global__ void settle_kernel() {}
+
 // One block: the sequences' new lengths and what is left of the stack.  A step whose tables have a status records nothing.
 __global__ void __launch_bounds__(TB) page_advance_kernel(const int32_t* slots, const int32_t* fresh, int n_seqs, int32_t* lengths,
                                                           int n_slots, int32_t* n_free, int page_size, const int32_t* status) {
@@ -272,6 +275,12 @@ extern "C" int sb_page_tables(const SbPageTables* args, cudaStream_t stream) {
   const long chunks = (a.max_rows + CHUNK - 1) / CHUNK + ((long)a.max_pages + CHUNK - 1) / CHUNK;
   sb_launch<SB_K_OTHER>(page_tables_kernel, dim3((unsigned)(chunks < 256 ? chunks : 256)), dim3(TB), smem, stream, a);
   SB_CHECK_LAUNCH(who);
+  return SB_OK;
+}
+
+extern "C" int sb_page_tables_settle(cudaStream_t stream) {
+  sb_launch<0>(settle_kernel, dim3(1), dim3(32), 0, stream);
+  SB_CHECK_LAUNCH("sb_page_tables_settle");
   return SB_OK;
 }
 

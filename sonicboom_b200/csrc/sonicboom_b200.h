@@ -553,6 +553,9 @@ typedef struct SbPageTables {
   int n_seqs, n_slots, width, n_pages, page_size, max_rows, max_pages, max_new, max_len;
 } SbPageTables;
 int sb_page_tables(const SbPageTables* args, sb_stream_t stream);
+/* A launch that starts only when all before it is over, and lets nothing start before it is over itself: between sb_page_tables and
+ * kernels that read a plan ahead of their wait for the kernel before them (sb_attention and sb_rope_store of few rows, sb_attention_f32). */
+int sb_page_tables_settle(sb_stream_t stream);
 /* The step that these tables described has run: lengths grow, n_free shrinks (neither where status is not 0). */
 int sb_page_advance(const int32_t* slots, const int32_t* fresh, int n_seqs, int32_t* lengths, int n_slots, int32_t* n_free, int page_size,
                     const int32_t* status, sb_stream_t stream);

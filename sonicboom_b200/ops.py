@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import weakref
 
 import torch
 
@@ -110,10 +111,39 @@ def _check(rc: int, what: str, launches: int = 1) -> None:
     LAUNCHES += launches
 
 
+_unsettled: dict = {}    # id -> weak reference of the PageTables that a kernel has written and no kernel has settled
+_unsettled_from = _unsettled_to = 0        # their arrays lie between these addresses
+
+
 def _i32(t, what):
     if t.dtype != torch.int32:
         raise KernelError(f"{what} must be int32, got {t.dtype}")
-    return _ptr(t)
+    address = _ptr(t)
+    if _unsettled_from <= address < _unsettled_to:
+        _settle(address)
+    return address
+
+
+def _note_unsettled(tables=None) -> None:
+    """Notes tables that a kernel is writing (None: some of those noted are settled or gone)."""
+    global _unsettled_from, _unsettled_to
+    if tables is not None:
+        _unsettled[id(tables)] = tables.ref
+    live = [t for t in (ref() for ref in _unsettled.values()) if t is not None]
+    _unsettled_from, _unsettled_to = min((t.start for t in live), default=0), max((t.end for t in live), default=0)
+
+
+def _settle(address: int) -> None:
+    """Kernels may read a plan's arrays ahead of their wait for the kernel before them: plans come from the host, complete before a
+    step's first kernel.  One that `page_tables` has made is not, so the first call that takes one of its arrays by way of `_i32` (the
+    kernels that wait first take them otherwise) launches a kernel ahead of its own that starts late and lets nothing start early."""
+    for key, ref in list(_unsettled.items()):
+        tables = ref()
+        if tables is None or tables.start <= address < tables.end:
+            if tables is not None:
+                _check(lib().sb_page_tables_settle(_stream()), "page_tables (settle)")
+            del _unsettled[key]
+    _note_unsettled()
 
 
 def embed(tokens: torch.Tensor, table: torch.Tensor, out: torch.Tensor,
@@ -417,7 +447,9 @@ def rotation_table(row_pos: torch.Tensor, inv_freq: torch.Tensor, rotary_dim: in
     """[rows, rotary_dim] float32: cosines, then sines, of every row's position times `inv_freq`."""
     assert inv_freq.dtype == torch.float32 and inv_freq.numel() >= rotary_dim // 2
     out = torch.empty((row_pos.numel(), rotary_dim), dtype=torch.float32, device=row_pos.device)
-    _check(lib().sb_rotation_table(_i32(row_pos, "row_pos"), row_pos.numel(), rotary_dim, _ptr(inv_freq), _ptr(out), _stream()),
+    if row_pos.dtype != torch.int32:
+        raise KernelError(f"row_pos must be int32, got {row_pos.dtype}")
+    _check(lib().sb_rotation_table(_ptr(row_pos), row_pos.numel(), rotary_dim, _ptr(inv_freq), _ptr(out), _stream()),
            "rotation table")
     return out
 
@@ -898,6 +930,8 @@ class PageTables:
         self.seq_row0.zero_(), self.page_off.zero_(), self.status.zero_()
         self.n_seqs, self.n_rows, self.max_pages, self.page_size = max_seqs, max_rows, max_pages, page_size
         self.device, self.index = flat.device, flat.get_device()
+        self.start, self.end = flat.data_ptr(), self.status.data_ptr()           # of the arrays that a step's kernels read
+        self.ref = weakref.ref(self)
         self.max_new = self.max_len = 0
         self.groups = [TableGroup(self.page_off, self.page_ids, page_size)]
         self._scratch = []
@@ -935,8 +969,9 @@ def page_tables(slots: torch.Tensor, new: torch.Tensor, lengths: torch.Tensor, t
     (`tables.check()` raises it).  Nothing is taken until `page_advance` records the step; called again before that, it gives the
     same pages.  All arrays int32.
 
-    Kernels that read a plan ahead of their wait for the kernel before them (`attention` and `rope_store` of few rows) must not come
-    directly behind this one; those over an 8-bit cache and `rotation_table` may."""
+    The operators over an 8-bit cache and `rotation_table` take the result as it is.  Ahead of the first other one that takes it
+    (`attention`, `rope_store`: their kernels read a plan while the kernel before them may still run) an empty kernel is launched
+    that keeps the two apart."""
     what, n, shape = "page_tables", tables.n_seqs, table.shape
     index = _device_of(lengths, what)
     if not slots.numel() == new.numel() == n:
@@ -953,6 +988,8 @@ def page_tables(slots: torch.Tensor, new: torch.Tensor, lengths: torch.Tensor, t
     if max_len != tables.max_len:                # the list is no longer than this: room that kernels need for each of its pages
         tables.groups[0].page_ids = tables.page_ids[:tables.n_seqs * -(-max_len // tables.page_size)]
     tables.max_new, tables.max_len = max_new, max_len
+    if id(tables) not in _unsettled or _unsettled[id(tables)] is not tables.ref:
+        _note_unsettled(tables)
     return tables
 
 
@@ -962,9 +999,12 @@ def page_advance(slots: torch.Tensor, new: torch.Tensor, lengths: torch.Tensor, 
     index = _device_of(lengths, "page_advance")
     if not slots.numel() == new.numel() == tables.n_seqs or n_free.numel() != 1:
         raise KernelError(f"page_advance: {slots.numel()} slots, {new.numel()} counts, tables for {tables.n_seqs} requests")
-    _addresses("page_advance", index, slots, new, n_free, tables.status)
-    _check(lib().sb_page_advance(_i32(slots, "slots"), _i32(new, "new"), tables.n_seqs, _i32(lengths, "lengths"), lengths.numel(),
-                                 _i32(n_free, "n_free"), tables.page_size, _i32(tables.status, "status"), _stream()), "page_advance")
+    for t in (slots, new, lengths, n_free):
+        if t.dtype is not _I32T:
+            raise KernelError(f"page_advance: all arrays are int32, got {t.dtype}")
+    named, brought, held, top, status = _addresses("page_advance", index, slots, new, lengths, n_free, tables.status)
+    _check(lib().sb_page_advance(named, brought, tables.n_seqs, held, lengths.numel(), top, tables.page_size, status, _stream_of(index)),
+           "page_advance")
 
 
 def page_release(slots: torch.Tensor, lengths: torch.Tensor, table: torch.Tensor, free: torch.Tensor, n_free: torch.Tensor,
@@ -973,10 +1013,12 @@ def page_release(slots: torch.Tensor, lengths: torch.Tensor, table: torch.Tensor
     index = _device_of(lengths, "page_release")
     if table.dim() != 2 or lengths.numel() != table.shape[0] or n_free.numel() != 1:
         raise KernelError(f"page_release: {lengths.numel()} lengths, a table of {tuple(table.shape)}, {n_free.numel()} counts of free pages")
-    _addresses("page_release", index, slots, table, free, n_free)
-    _check(lib().sb_page_release(_i32(slots, "slots"), slots.numel(), _i32(lengths, "lengths"), _i32(table, "table"), table.shape[0],
-                                 table.shape[1], _i32(free, "free"), free.numel(), _i32(n_free, "n_free"), page_size, _stream()),
-           "page_release")
+    for t in (slots, lengths, table, free, n_free):
+        if t.dtype is not _I32T:
+            raise KernelError(f"page_release: all arrays are int32, got {t.dtype}")
+    named, held, pages, stack, top = _addresses("page_release", index, slots, lengths, table, free, n_free)
+    _check(lib().sb_page_release(named, slots.numel(), held, pages, table.shape[0], table.shape[1], stack, free.numel(), top, page_size,
+                                 _stream_of(index)), "page_release")
 
 
 def sample_params_size() -> int:

@@ -125,3 +125,44 @@ def test_scratch_memory_of_tables_that_grow_step_by_step():
         assert got.numel() >= n and sum(b.numel() for b in t._scratch) < 4 * n
         assert t.scratch(n // 2, "cpu") is got
     assert t._scratch[0] is first and t.scratch(0, "cpu") is None and len(t._scratch) <= 9
+
+
+# ------------------------------------------------------------------------------------------------ plans made on the device
+def make_tables(n=2, tables=None):
+    tables = tables or ops.PageTables(n, 4, 8, "cpu")
+    one = torch.ones(n, dtype=torch.int32)
+    return ops.page_tables(i32(list(range(n))), one, one, torch.zeros(n, 4, dtype=torch.int32), i32([0] * 8), i32([8]), tables, 1, 256)
+
+
+def test_kernels_that_read_a_plan_early_are_kept_apart_from_the_one_that_makes_it(recorder, monkeypatch):
+    """Once for every making of the tables, ahead of the first kernel that may read one of their arrays before its wait; not for
+    kernels that wait first."""
+    monkeypatch.setattr(ops, "_ptr", lambda t: None if t is None else t.data_ptr())
+    monkeypatch.setattr(ops, "_stream", lambda: 0)
+    names = lambda: [name for name, _ in recorder.calls if not name.endswith("_bytes")]                      # noqa: E731
+    q, out = (torch.zeros(4, 4, 22, dtype=torch.bfloat16) for _ in range(2))
+
+    def store(t):
+        g = t.groups[0]
+        ops.rope_store(torch.zeros(4, 8 * 22), 4, 2, 22, 0, torch.ones(11), t.row_seq, t.row_pos, g.page_off, g.page_ids, 64,
+                       torch.zeros(8, 2, 2, 64, 22, dtype=torch.bfloat16), q)
+
+    t, other = make_tables(), make_tables()
+    ops.rotation_table(t.row_pos, torch.ones(8), 16)
+    attend(t, kernel="plain")
+    ops.page_advance(i32([0, 1]), i32([1, 1]), i32([1, 1]), i32([8]), t)
+    assert "sb_page_tables_settle" not in names() and len(names()) == 5
+    recorder.calls.clear()
+    store(t)
+    store(t)
+    assert names() == ["sb_page_tables_settle", "sb_rope_store", "sb_rope_store"]
+    recorder.calls.clear()
+    ops.attention(q, out, other, 0, torch.zeros(8, 2, 2, 64, 22), 4, 2, 22, 0, 0.1, kernel="plain")
+    assert names() == ["sb_page_tables_settle", "sb_attention_plain"]
+    recorder.calls.clear()
+    make_tables(tables=t)
+    store(t)
+    del t, other
+    make_tables()                                                               # gone before anything reads them
+    ops.rotation_table(i32([0]), torch.ones(8), 16)
+    assert names() == ["sb_page_tables", "sb_page_tables_settle", "sb_rope_store", "sb_page_tables", "sb_rotation_table"]

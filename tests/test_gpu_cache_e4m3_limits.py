@@ -95,3 +95,57 @@ def test_a_retired_row_leaves_its_pages_alone(model_dirs, dtype):
     assert all(0 <= t for t in tokens[3:])
     loop.close()
     assert [eng.length(s) for s in slots] == [73, 64, 8, 32]
+
+
+# ------------------------------------------------------------------------------------------------ plans made on the device
+@pytest.mark.parametrize("dtype,hd", [(torch.bfloat16, 64), (torch.float32, 64), (torch.float32, 22)])
+def test_a_bfloat16_or_float32_cache_under_tables_made_on_the_device(dtype, hd):
+    """`rope_store` and `attention` directly behind `page_tables`, eagerly and in a replayed graph, token by token across page ends:
+    the same bits as with a plan from the host."""
+    hq, hkv, n_pages = 4, 2, 8
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=DEV)                       # noqa: E731
+    g = torch.Generator().manual_seed(hd)
+    slots, new, lengths = i32([2, 0]), i32([1, 1]), i32([60, 9, 127])
+    table, free, n_free = i32([[0, -1, -1], [-1] * 3, [1, 2, -1]]), i32([7, 6, 5, 4, 3, 0, 0, 0]), i32([5])
+    caches = [torch.randn(n_pages, 2, hkv, 64, hd, generator=g).to(dtype).to(DEV) for _ in range(1)]
+    caches.append(caches[0].clone())
+    inv = torch.ones(hd // 2, device=DEV)
+    t = ops.PageTables(2, 2, 6, DEV)
+    x, q = torch.empty(2, (hq + 2 * hkv) * hd, device=DEV), torch.empty(2, hq, hd, dtype=dtype, device=DEV)
+    outs = [torch.empty(2, hq * hd, dtype=dtype, device=DEV) for _ in range(2)]
+
+    def one_step(plan, cache, out):
+        group = plan.groups[0]
+        ops.rope_store(x, hq, hkv, hd, 0, inv, plan.row_seq, plan.row_pos, group.page_off, group.page_ids, 64, cache, q)
+        ops.attention(q, out, plan, 0, cache, hq, hkv, hd, 0, 0.125)
+
+    def device_step():
+        ops.page_tables(slots, new, lengths, table, free, n_free, t, 1, 192)
+        one_step(t, caches[0], outs[0])
+        ops.page_advance(slots, new, lengths, n_free, t)
+
+    state = [caches[0], lengths, table, n_free]
+    kept = [v.clone() for v in state]
+    x.zero_()
+    before = ops.LAUNCHES
+    device_step()                                                               # builds what is built lazily; nothing of it stays
+    assert ops.LAUNCHES - before == 5                                           # the one that keeps them apart among them
+    torch.cuda.synchronize()
+    for v, was in zip(state, kept):
+        v.copy_(was)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        device_step()
+    pages, pos = [[1, 2], [0]], [127, 60]
+    for step in range(12):
+        x.copy_(torch.randn(x.shape, generator=g))
+        device_step() if step % 3 == 2 else graph.replay()
+        for i in range(2):
+            if pos[i] % 64 == 0:
+                pages[i].append(3 + sum(len(p) for p in pages) - 3)             # the stack's top: 3, then 4, ...
+        plan = Plan([1, 1], pos, pages)
+        plan.max_len = 192
+        one_step(plan, caches[1], outs[1])
+        pos = [p + 1 for p in pos]
+        assert torch.equal(outs[0], outs[1]) and torch.equal(caches[0], caches[1]), step
+        assert lengths.tolist() == [pos[1], 9, pos[0]]
