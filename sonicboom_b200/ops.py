@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import struct
 import weakref
 
 import torch
@@ -707,7 +708,20 @@ E4M3 = torch.float8_e4m3fn
 
 
 _I32T, _F32T = torch.int32, torch.float32
-_pack_store, _pack_tables, _pack_attention = (_abi.pack[name] for name in ("SbStoreE4m3", "SbPageTables", "SbAttentionE4m3"))
+
+
+def _packer(name):
+    pack = _abi.pack[name]
+
+    def packed(*values):
+        try:
+            return pack(*values)
+        except struct.error as e:
+            raise KernelError(f"{name}: {e}") from None
+    return packed
+
+
+_pack_store, _pack_tables, _pack_attention = (_packer(name) for name in ("SbStoreE4m3", "SbPageTables", "SbAttentionE4m3"))
 
 
 def _device_of(t, what) -> int:

@@ -166,3 +166,21 @@ def test_kernels_that_read_a_plan_early_are_kept_apart_from_the_one_that_makes_i
     make_tables()                                                               # gone before anything reads them
     ops.rotation_table(i32([0]), torch.ones(8), 16)
     assert names() == ["sb_page_tables", "sb_page_tables_settle", "sb_rope_store", "sb_page_tables", "sb_rotation_table"]
+
+
+def test_numbers_that_no_record_holds_are_refused(recorder):
+    """Beyond 32 bits, or no whole numbers: the module's own error, and nothing is launched."""
+    tables = ops.PageTables(2, 4, 8, "cpu")
+    one, state = i32([1, 1]), (i32([0, 0]), torch.zeros(2, 4, dtype=torch.int32), i32([0] * 8), i32([8]))
+    for max_new, max_len in ((2 ** 31, 256), (1, 2 ** 31), (1, 2.5)):
+        with pytest.raises(ops.KernelError, match="SbPageTables"):
+            ops.page_tables(i32([0, 1]), one, *state, tables, max_new, max_len)
+    plan = Plan([1], [5], [[0]])
+    for window in (2 ** 31, 0.5):
+        with pytest.raises(ops.KernelError, match="SbAttentionE4m3"):
+            attend(plan, window=window)
+    plan.max_new = 2 ** 31
+    cache = torch.zeros(4, 2, 2, 64, 64, dtype=torch.uint8).view(torch.float8_e4m3fn)
+    with pytest.raises(ops.KernelError, match="SbStoreE4m3"):
+        ops.rope_store_e4m3(torch.zeros(1, 8 * 64), 4, 2, 64, 0, None, plan, 0, cache, torch.ones(4, 2, 2), torch.zeros(1, 4, 64))
+    assert not [name for name, _ in recorder.calls if not name.endswith("_bytes")]
