@@ -32,15 +32,21 @@ class DevicePages:
         """Room for a step's tables: `max_seqs` requests, `max_rows` rows of all of them and `max_pages` pages (as many as the
         requests can have)."""
         most = min(self.n_pages, max_seqs * self.pages_per_slot)
-        return ops.PageTables(max_seqs, max_rows, max_pages or most, self.lengths.device, self.page_size)
+        return ops.PageTables(max_seqs, max_rows, most if max_pages is None else max_pages, self.lengths.device, self.page_size)
+
+    def _check(self, tables: ops.PageTables) -> None:
+        if tables.page_size != self.page_size:
+            raise CacheError(f"tables for pages of {tables.page_size} tokens, these have {self.page_size}")
 
     def plan(self, slots: torch.Tensor, new: torch.Tensor, tables: ops.PageTables, max_new: int, max_len: int = 0) -> ops.PageTables:
         """The tables of a step in which the sequence in `slots[i]` gets `new[i]` tokens (see `ops.page_tables`)."""
+        self._check(tables)
         return ops.page_tables(slots, new, self.lengths, self.table, self.free, self.n_free, tables, max_new,
                                max_len or self.pages_per_slot * self.page_size)
 
     def advance(self, slots: torch.Tensor, new: torch.Tensor, tables: ops.PageTables) -> None:
         """That step has run."""
+        self._check(tables)
         ops.page_advance(slots, new, self.lengths, self.n_free, tables)
 
     def release(self, slots: torch.Tensor) -> None:

@@ -931,7 +931,8 @@ class PageTables:
     requests together: a plan that the kernels take.  Its addresses stay, so a captured graph may write and read it."""
 
     def __init__(self, max_seqs: int, max_rows: int, max_pages: int, device, page_size: int = 64):
-        assert min(max_seqs, max_rows, max_pages, page_size) > 0
+        if min(max_seqs, max_rows, max_pages, page_size) <= 0:
+            raise KernelError(f"tables with room for {max_seqs} requests, {max_rows} rows and {max_pages} pages of {page_size} tokens")
         sizes = [max_seqs + 1, max_seqs, max_rows, max_rows, max_rows, max_seqs + 1, max_pages, 1]
         starts = [0]
         for n in sizes:

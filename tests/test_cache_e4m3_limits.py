@@ -184,3 +184,24 @@ def test_numbers_that_no_record_holds_are_refused(recorder):
     with pytest.raises(ops.KernelError, match="SbStoreE4m3"):
         ops.rope_store_e4m3(torch.zeros(1, 8 * 64), 4, 2, 64, 0, None, plan, 0, cache, torch.ones(4, 2, 2), torch.zeros(1, 4, 64))
     assert not [name for name, _ in recorder.calls if not name.endswith("_bytes")]
+
+
+def test_device_pages_take_tables_of_their_own_page_size_only(recorder):
+    """Lengths, page lists and the stack count pages of one size."""
+    from sonicboom_b200.cache import CacheError, DevicePages
+    pages = DevicePages(4, 8, 4, "cpu", page_size=32)
+    slots, one = i32([0, 1]), i32([1, 1])
+    mine = pages.tables(2, 4)
+    assert mine.page_size == 32 and mine.max_pages == 8 and pages.tables(2, 4, 3).max_pages == 3
+    pages.plan(slots, one, mine, 1)
+    pages.advance(slots, one, mine)
+    other = ops.PageTables(2, 4, 8, "cpu")
+    for call in (lambda: pages.plan(slots, one, other, 1), lambda: pages.advance(slots, one, other)):
+        with pytest.raises(CacheError, match="tokens"):
+            call()
+    assert [name for name, _ in recorder.calls] == ["sb_page_tables", "sb_page_advance"]
+    with pytest.raises(ops.KernelError, match="room"):
+        pages.tables(2, 4, 0)
+    for sizes in ((0, 4, 4), (2, 0, 4), (2, 4, -1), (2, 4, 4, "cpu", 0)):
+        with pytest.raises(ops.KernelError, match="room"):
+            ops.PageTables(*sizes[:3], "cpu", *sizes[4:])
