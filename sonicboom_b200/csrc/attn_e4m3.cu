@@ -11,17 +11,20 @@
 // page's keys of the head, another its values, into the warp's own shared memory, and the next page's are asked for as soon as
 // the tile has been read.  (Copies of 16 bytes a lane, into registers or shared memory, kept the memory at 4.4 of the 6.1 TB/s
 // that bulk copies of the same pages reach: 64 sequences of 512 to 8,192 keys 78 to 80 us when bulk copies took 65.)
-// e4m3 to half is exact.  q is brought to halves with a power of two for each row: a bfloat16's 8 bits stay.  Weights are rounded
-// to halves (2^-11) after they were summed in float32, times 2^15 so that small ones stay normal numbers.  For float32 rows q and
-// the weights are two halves each, the second what the first left over (together within 2^-24 of a row's largest value, 2^-22
-// of a weight), and every product two.
+// e4m3 to half is exact.  q is brought to halves with a power of two for each row: a bfloat16's 8 bits stay down to 2^-17 of the
+// row's largest number, smaller ones are off by at most 2^-25 of it.  Weights are rounded to halves (2^-11 of a weight) after they
+// were summed in float32, times 2^15 so that those down to 2^-29 of the largest are normal numbers; smaller ones are off by at most
+// 2^-40 of it.  For float32 rows q and the weights are two halves each, the second what the first left over (together within 2^-24 of
+// a row's largest number, 2^-22 of a weight or 2^-40 of the largest), and every product two.
 //
 // Scales.  A page's key scale joins the score.  Its value scale 2^e joins the weight: with m the largest score so far and n the
 // largest of score + e, weights are exp2(s - m) in the sum and exp2(s + e - n) in the product with V, each at most 1, and
-// the two references meet when the partial results are merged.  So pages of very unequal scale lose nothing.
+// the two references meet when the partial results are merged.  "Largest" above is of the weights times their pages' scales that
+// a warp has met: a page whose share is 2^29 below another's loses bits, one 2^40 below counts as 0, also in a channel where the
+// other page holds zeros.  (The kernels over values and the plain one multiply in float32's or bfloat16's range.)
 //
-// A sequence's keys are cut into splits of whole pages by its own length alone, so a result depends on neither the batch nor
-// the pages' places: a block takes one split of one key/value head, warp w its pages w, w + 4, ..., merged in warp order; splits
+// A sequence's keys are cut into splits of whole pages by its own length alone, so this kernel's result depends on neither the batch
+// nor the pages' places: a block takes one split of one key/value head, warp w its pages w, w + 4, ..., merged in warp order; splits
 // are merged in ascending order by a second kernel.  (The block that is done last, by an arrival counter, took 3 us more than the
 // kernel's 2 at one sequence and as much more at 64; a cluster of the splits' blocks held shared memory for sequences with fewer
 // splits, 89 us when this took 65.)

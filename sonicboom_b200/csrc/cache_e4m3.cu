@@ -218,7 +218,8 @@ __global__ void __launch_bounds__(THREADS) store_many_kernel(const SbStoreE4m3 a
 
 // -------------------------------------------------------------------------------------- values
 // The pages of a step's sequences as values in bfloat16 or float32, one after another as the plan lists them: [place in
-// page_ids][k|v][head][position][hd], with `numbers` for the page list that says so.  Exact in either type (a number has four bits, the scale is a power of two).  What no row of
+// page_ids][k|v][head][position][hd], with `numbers` for the page list that says so.  Exact (a number has four bits, the scale is a power of two) but for bfloat16 at
+// scales below 2^-124, whose smallest numbers lie below bfloat16's smallest, 2^-133, and are rounded to it or to 0.  What no row of
 // the step sees (positions behind a sequence's end, before its first row's window) becomes 0, whatever the page holds there; pages
 // that lie wholly before the window are left out.  A sequence whose list ends before its last row gets rows of zeros in `out`, which
 // the attention of bfloat16 rows behind this kernel leaves alone; that of float32 rows goes row by row, and finds that the pages

@@ -508,10 +508,11 @@ typedef struct SbStoreE4m3 {
   int n_rows, n_seqs, max_new, n_q_heads, n_kv_heads, hd, rot, page_size, n_pages, q_dtype, n_sms;
 } SbStoreE4m3;
 int sb_rope_store_e4m3(const SbStoreE4m3* args, sb_stream_t stream);
-/* The pages of a step's sequences as values (exactly), one after another as page_ids [n_list] lists them, [k|v][kv head][position]
- * [hd] each, with the page list numbers [n_list] that says so; 0 at positions that no row of the step sees.  Pages wholly before the window are left out.  A sequence whose list ends
- * before its last row gets zeros in out [rows][n_q_heads * hd], of the values' dtype, and -1 as its pages' numbers: what attends to the
- * values leaves such rows alone, or finds nothing but zeros. */
+/* The pages of a step's sequences as values (exactly; in bfloat16 at scales from 2^-124 on), one after another as page_ids [n_list]
+ * lists them, [k|v][kv head][position][hd] each, with the page list numbers [n_list] that says so; 0 at positions that no row of the
+ * step sees.  Pages wholly before the window are left out.  A sequence whose list ends before its last row gets zeros in out [rows]
+ * [n_q_heads * hd], of the values' dtype, and -1 as its pages' numbers: what attends to the values leaves such rows alone, or finds
+ * nothing but zeros. */
 int sb_cache_e4m3_values(const int32_t* seq_row0, const int32_t* seq_pos0, int n_seqs, int max_len, const int32_t* page_off,
                          const int32_t* page_ids, int n_list, int page_size, const void* cache, const float* scales, int n_pages,
                          int n_q_heads, int n_kv_heads, int hd, int window, void* values, int dtype, int32_t* numbers, void* out,

@@ -869,8 +869,15 @@ def attention_e4m3(q: torch.Tensor, out: torch.Tensor, plan, group_index: int, c
 
     Head sizes in steps of 16 up to 256 with pages of 64 keys run on tensor cores (built for the head size at first use): "few"
     reads the pages as they are, float32 rows and weights as two halves each; bfloat16 rows in such numbers that this is slower
-    have the step's pages brought to values first (exact, in the plan's scratch memory) and run `attention`, and so does float32
-    at other head sizes that are multiples of 4 up to 256: "values".  Anything else runs the "plain" kernel.  `kernel` names one."""
+    have the step's pages brought to values first (exact from scales of 2^-124 on, in the plan's scratch memory) and run `attention`,
+    and so does float32 at other head sizes that are multiples of 4 up to 256: "values".  Anything else runs the "plain" kernel.
+    `kernel` names one.
+
+    The choice goes by the whole step, so a sequence's bits may change with what else the step holds; those of one kernel do not
+    ("few", "plain").  Keys and values that a row does not see may be NaN; only where bfloat16 rows run over "values" does a value's NaN
+    reach rows before it that share its block, as in `attention`.  "few" counts a page as nothing for a row where its weight
+    times its scale lies 2^40 below another's.  Scratch memory (for float32 rows up to 4 GiB of partial results) is the plan's: two
+    calls that run at the same time need plans of their own."""
     global LAUNCHES
     what, n, g, dtype = "attention_e4m3", plan.n_rows, plan.groups[group_index], q.dtype
     index = _device_of(q, what)

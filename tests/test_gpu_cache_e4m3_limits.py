@@ -149,3 +149,55 @@ def test_a_bfloat16_or_float32_cache_under_tables_made_on_the_device(dtype, hd):
         pos = [p + 1 for p in pos]
         assert torch.equal(outs[0], outs[1]) and torch.equal(caches[0], caches[1]), step
         assert lengths.tolist() == [pos[1], 9, pos[0]]
+
+
+# ------------------------------------------------------------------------------------------------ how far numbers may lie apart
+@pytest.mark.parametrize("kernel", ["few", "plain", "values"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("apart", [10, 29, 35, 50])
+def test_pages_whose_scales_lie_far_apart(kernel, dtype, apart):
+    """One page has 2^apart in its first channel, another one, that the same warp takes after it, 1 in its second; every key counts
+    alike.  Weights times scales are halves in the "few" kernel: within 2^-40 of the largest, whatever the other page's is."""
+    hq = hkv = 1
+    hd, n_pages, length = 64, 36, 2200                                          # splits of eight pages from 2,049 keys on
+    cache = torch.zeros(n_pages, 2, hkv, 64, hd, device=DEV)
+    scales = torch.full((n_pages, 2, hkv), 2.0 ** -126, device=DEV)
+    for page, channel, e in ((0, 0, apart - 8), (4, 1, -8)):
+        cache[page, 1, 0, :, channel] = 256.0
+        scales[page, 1] = 2.0 ** e
+    plan = Plan([1], [length - 1], [list(range(-(-length // 64)))])
+    out = torch.empty(1, hd, dtype=dtype, device=DEV)
+    ops.attention_e4m3(torch.ones(1, 1, hd, dtype=dtype, device=DEV), out, plan, 0, cache.to(torch.float8_e4m3fn), scales, hq, hkv, hd, 0, 0.0, kernel)
+    got, share = out.double().cpu()[0], 64 / length
+    # sums in 32 bits of `length` terms and the result's rounding; a page's 64 weights are off by 2^-40 of the largest, which is 2^apart
+    rounding = 2.0 ** -8 * (dtype == torch.bfloat16) + 2 * length * 2.0 ** -24
+    weight = 2.0 ** -8 if dtype == torch.bfloat16 else 2.0 ** -20               # relative, of a weight that is a normal number
+    assert abs(float(got[0]) - share * 2.0 ** apart) <= (rounding + weight) * share * 2.0 ** apart
+    lost = share * 2.0 ** (apart - 40) if kernel == "few" else 0.0
+    assert abs(float(got[1]) - share) <= (rounding + weight) * share + lost
+    assert bool((got[2:] == 0).all())
+
+
+@pytest.mark.parametrize("kind", [0, 1])
+@pytest.mark.parametrize("dtype,kernel", [(torch.bfloat16, "values"), (torch.float32, "values"), (torch.float32, "plain"), (torch.bfloat16, "plain")])
+@pytest.mark.parametrize("hd", [64, 48])
+def test_a_nan_among_many_new_rows(dtype, kernel, kind, hd):
+    """Every row that sees it becomes NaN, no row of another sequence; a row before it only where bfloat16 rows run over values and it
+    is a value's."""
+    hq, hkv, n, pos0, bad = 4, 2, 40, 70, 90
+    cache, scales = ones(4, hkv, 64, hd)
+    cache.view(torch.uint8)[1, kind, 0, bad - 64, 5] = 0x7f
+    plan = Plan([n, n], [pos0, pos0], [[0, 1], [2, 3]])
+    out = torch.empty(2 * n, hq * hd, dtype=dtype, device=DEV)
+    ops.attention_e4m3(torch.ones(2 * n, hq, hd, dtype=dtype, device=DEV), out, plan, 0, cache, scales, hq, hkv, hd, 0, 0.1, kernel)
+    got = out.view(2 * n, hq, hd).float().cpu()
+    sees = torch.arange(pos0, pos0 + n) >= bad
+    seen = got[:n, :2][sees]
+    assert bool((seen if kind == 0 else seen[..., 5]).isnan().all())
+    fine = torch.ones(2 * n, hq, hd, dtype=torch.bool)
+    fine[:n, :2] = ~sees[:, None, None]
+    if kind == 1:
+        fine[..., [d for d in range(hd) if d != 5]] = True
+        if dtype == torch.bfloat16 and kernel == "values":
+            fine[:n, :2, 5] = False
+    assert float((got[fine] - 1).abs().max()) <= 2.0 ** -7
