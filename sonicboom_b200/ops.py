@@ -129,7 +129,7 @@ def _note_unsettled(tables=None) -> None:
     """Notes tables that a kernel is writing (None: some of those noted are settled or gone)."""
     global _unsettled_from, _unsettled_to
     if tables is not None:
-        _unsettled[id(tables)] = tables.ref
+        tables.settled, _unsettled[id(tables)] = False, weakref.ref(tables)
     live = [t for t in (ref() for ref in _unsettled.values()) if t is not None]
     _unsettled_from, _unsettled_to = min((t.start for t in live), default=0), max((t.end for t in live), default=0)
 
@@ -143,6 +143,7 @@ def _settle(address: int) -> None:
         if tables is None or tables.start <= address < tables.end:
             if tables is not None:
                 _check(lib().sb_page_tables_settle(_stream()), "page_tables (settle)")
+                tables.settled = True
             del _unsettled[key]
     _note_unsettled()
 
@@ -708,20 +709,7 @@ E4M3 = torch.float8_e4m3fn
 
 
 _I32T, _F32T = torch.int32, torch.float32
-
-
-def _packer(name):
-    pack = _abi.pack[name]
-
-    def packed(*values):
-        try:
-            return pack(*values)
-        except struct.error as e:
-            raise KernelError(f"{name}: {e}") from None
-    return packed
-
-
-_pack_store, _pack_tables, _pack_attention = (_packer(name) for name in ("SbStoreE4m3", "SbPageTables", "SbAttentionE4m3"))
+_pack_store, _pack_tables, _pack_attention = (_abi.pack[name] for name in ("SbStoreE4m3", "SbPageTables", "SbAttentionE4m3"))
 
 
 def _device_of(t, what) -> int:
@@ -800,9 +788,12 @@ def rope_store_e4m3(qkv: torch.Tensor, n_q_heads: int, n_kv_heads: int, head_dim
     rows, kept, kept_scales, q, row0, pos0, off, ids = _addresses(what, index, qkv, cache, scales, q_out, *_check_plan(what, plan, g))
     if _overlap(qkv, rows, q_out, q):
         raise KernelError(f"{what}: the rows and q_out share memory")
-    _check(lib().sb_rope_store_e4m3(_pack_store(
-        rows, turn, row0, pos0, off, ids, kept, kept_scales, q, n, plan.n_seqs, plan.max_new, n_q_heads, n_kv_heads, head_dim, rotary_dim,
-        g.page_size, cache.shape[0], _code(q_out.dtype), _sm_count(index)), _stream_of(index)), what)
+    try:
+        record = _pack_store(rows, turn, row0, pos0, off, ids, kept, kept_scales, q, n, plan.n_seqs, plan.max_new, n_q_heads, n_kv_heads, head_dim,
+                             rotary_dim, g.page_size, cache.shape[0], _code(q_out.dtype), _sm_count(index))
+    except struct.error as e:
+        raise KernelError(f"{what}: SbStoreE4m3: {e}") from None
+    _check(lib().sb_rope_store_e4m3(record, _stream_of(index)), what)
     return q_out
 
 
@@ -902,10 +893,14 @@ def attention_e4m3(q: torch.Tensor, out: torch.Tensor, plan, group_index: int, c
     if few:
         al = attention_lib(head_dim)
         scratch = plan.scratch(_e4m3_scratch_bytes(head_dim, n, n_q_heads, plan.max_len), q.device)
-        rc = al.sb_attention_e4m3(_pack_attention(
-            rows, to, row0, pos0, off, ids, kept, kept_scales, scratch.data_ptr() if scratch is not None else 0,
-            scratch.numel() if scratch is not None else 0, _code(dtype), n, plan.n_seqs, plan.max_new, plan.max_len, g.page_size,
-            cache.shape[0], n_q_heads, n_kv_heads, head_dim, window, scale), _stream_of(index))
+        try:
+            record = _pack_attention(
+                rows, to, row0, pos0, off, ids, kept, kept_scales, scratch.data_ptr() if scratch is not None else 0,
+                scratch.numel() if scratch is not None else 0, _code(dtype), n, plan.n_seqs, plan.max_new, plan.max_len, g.page_size,
+                cache.shape[0], n_q_heads, n_kv_heads, head_dim, window, scale)
+        except struct.error as e:
+            raise KernelError(f"{what}: SbAttentionE4m3: {e}") from None
+        rc = al.sb_attention_e4m3(record, _stream_of(index))
         if rc != 0:
             raise KernelError(f"{what}: {al.sb_last_error().decode()}")
         LAUNCHES += 1 if scratch is None else 2
@@ -953,7 +948,7 @@ class PageTables:
         self.n_seqs, self.n_rows, self.max_pages, self.page_size = max_seqs, max_rows, max_pages, page_size
         self.device, self.index = flat.device, flat.get_device()
         self.start, self.end = flat.data_ptr(), self.status.data_ptr()           # of the arrays that a step's kernels read
-        self.ref = weakref.ref(self)
+        self.settled = True                                                      # whether a step's kernels may read them early
         self.max_new = self.max_len = 0
         self.groups = [TableGroup(self.page_off, self.page_ids, page_size)]
         self._scratch = []
@@ -1004,13 +999,16 @@ def page_tables(slots: torch.Tensor, new: torch.Tensor, lengths: torch.Tensor, t
             or n_free.dtype is not _I32T:
         raise KernelError(f"{what}: all arrays are int32")
     named, brought, held, pages, stack, top = _addresses(what, index, slots, new, lengths, table, free, n_free)
-    _check(lib().sb_page_tables(_pack_tables(
-        named, brought, held, pages, stack, top, *tables._pointers, n, *shape, free.numel(), tables.page_size, tables.n_rows, tables.max_pages,
-        max_new, max_len), _stream_of(index)), what)
+    try:
+        record = _pack_tables(named, brought, held, pages, stack, top, *tables._pointers, n, *shape, free.numel(), tables.page_size, tables.n_rows,
+                              tables.max_pages, max_new, max_len)
+    except struct.error as e:
+        raise KernelError(f"{what}: SbPageTables: {e}") from None
+    _check(lib().sb_page_tables(record, _stream_of(index)), what)
     if max_len != tables.max_len:                # the list is no longer than this: room that kernels need for each of its pages
         tables.groups[0].page_ids = tables.page_ids[:tables.n_seqs * -(-max_len // tables.page_size)]
     tables.max_new, tables.max_len = max_new, max_len
-    if id(tables) not in _unsettled or _unsettled[id(tables)] is not tables.ref:
+    if tables.settled:
         _note_unsettled(tables)
     return tables
 
