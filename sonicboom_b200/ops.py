@@ -798,12 +798,13 @@ def rope_store_e4m3(qkv: torch.Tensor, n_q_heads: int, n_kv_heads: int, head_dim
 
 
 def _reads_pages_directly(plan, dtype, n_q_heads: int, n_kv_heads: int, head_dim: int, n_sms: int) -> bool:
-    """Whether rows attend to 8-bit pages as they are: sixteen bfloat16 rows of a key/value head at a time, the pages read and
-    converted again for every sixteen; or to their values, written out first, 256 rows at a time.  The first one's time grows with
-    rows x keys, the second one's with the keys that a block walks alone.  In us, fitted to 1 and 8 sequences, 7 to 448 rows, 100
-    to 16,000 keys, head sizes 64 and 128 (the choice is the faster one in all but near ties: 8 sequences of 112 rows over 900
-    keys 30 us and 26 us, 63 rows over 4,000 keys 47 us and 86 us, one of 448 rows over 4,000 keys 41 us and 75 us).
-    float32 rows do, eight at a time, as far as a grid and a few GB of partial rows go: their other way is 2.5 to 40 times slower."""
+    """Whether rows attend to 8-bit pages as they are ("few"): sixteen bfloat16 rows of a key/value head at a time, the pages read and
+    converted again for every sixteen; or to their values ("values"), written out first, 256 rows at a time.  The first one's time
+    grows with rows x keys, the second one's with the keys that a block walks alone.  In us, fitted to 1 and 8 sequences, 7 to 448 rows,
+    100 to 16,000 keys, head sizes 64 and 128; few / values at 28/4 heads of 128: 8 sequences of 112 rows over 900 keys 30 / 26, of 63 rows
+    over 4,000 keys 47 / 86, one of 448 rows over 4,000 keys 41 / 75.  Of 144 such sizes the choice is the slower one at six, by 3 to 36 %
+    (the most at 8 sequences of 444 rows over 16,000 keys, 6/1 heads of 64: 184 / 249).
+    float32 rows do, eight at a time, as far as a grid and 4 GiB of partial rows go: their other way is 2.5 to 40 times slower."""
     rows, keys = plan.max_new * (n_q_heads // n_kv_heads), plan.max_len
     if rows <= 16:
         return True
