@@ -130,6 +130,8 @@ def _note_unsettled(tables=None) -> None:
     global _unsettled_from, _unsettled_to
     if tables is not None:
         tables.settled, _unsettled[id(tables)] = False, weakref.ref(tables)
+    for key in [k for k, ref in _unsettled.items() if ref() is None]:
+        del _unsettled[key]
     live = [t for t in (ref() for ref in _unsettled.values()) if t is not None]
     _unsettled_from, _unsettled_to = min((t.start for t in live), default=0), max((t.end for t in live), default=0)
 

@@ -205,3 +205,10 @@ def test_device_pages_take_tables_of_their_own_page_size_only(recorder):
     for sizes in ((0, 4, 4), (2, 0, 4), (2, 4, -1), (2, 4, 4, "cpu", 0)):
         with pytest.raises(ops.KernelError, match="room"):
             ops.PageTables(*sizes[:3], "cpu", *sizes[4:])
+
+
+def test_tables_that_are_gone_are_forgotten(recorder):
+    for _ in range(50):
+        make_tables()
+    kept = make_tables()
+    assert len(ops._unsettled) == 1 and ops._unsettled_from == kept.start and ops._unsettled_to == kept.end
